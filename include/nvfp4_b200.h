@@ -371,6 +371,106 @@ int nvfp4_rmsnorm_bwd(const void* x, int x_is_f32, const float* weight, const fl
 int nvfp4_rotary_bf16(const void* q, void* q_out, int q_heads, const void* k, void* k_out, int k_heads, int64_t rows,
                       int64_t seq, int head_dim, const float* cosine, const float* sine, int backward, void* stream);
 
+/*
+ * AdamW over many tensors at once.  For every tensor, with t its number of steps, all in fp32, every product, sum, quotient
+ * and root rounded by itself:
+ *   g' = c g;  m' = b1 m + (1 - b1) g';  v' = b2 v + ((1 - b2) g') g'
+ *   p' = p (1 - lr wd) - (lr / (1 - b1^t)) (m' / (sqrt(v') / sqrt(1 - b2^t) + eps))
+ * param and grad are both fp32 (is_f32 != 0) or both bf16, contiguous, n elements each.
+ *   state_bits 32: first = m, second = v, fp32 [n]; the scales are not looked at.
+ *   state_bits 8:  first and second hold m and sqrt(v) as E4M3 codes [ceil(n / 256) * 256], first_scale and second_scale one
+ *     E8M0 power of two per 256 codes [ceil(n / 256)] (byte 255: the block is NaN, which is what a block with an element
+ *     of 2^51 or more, an infinity or a NaN becomes).  All zero is a valid start.  Codes are rounded stochastically: Philox4x32-10 with
+ *     key philox_seed and counter (counter_base + element / 8, philox_offset), 16 bits for each of eight elements in
+ *     order, low half of a word first; sqrt(v) takes the same 16 bits reversed.
+ * Clipping: c = min(1, max_norm / (norm + 1e-6)) with norm from `sumsq_parts` (n_parts doubles that nvfp4_sumsq left) or
+ * from the device word `norm`; c = 1 when both are NULL.  norm_out, if not NULL, receives the norm.
+ * `tensors` and `hypers` are HOST arrays, read before the call returns; up to 8 hypers, which tensors name by index.
+ * Tensors must not overlap.  No counterpart in the reference, which steps torch.optim.AdamW after
+ * clip_grad_norm_ (nvfp4_train.py:159-185).
+ */
+typedef struct {
+  void* param;
+  const void* grad;
+  void* first;
+  void* second;
+  void* first_scale;
+  void* second_scale;
+  int64_t n;
+  uint64_t counter_base;
+  int32_t hyper;
+} nvfp4_adamw_tensor;
+typedef struct {
+  float decay;                /* 1 - lr wd */
+  float beta1, rest1;         /* b1, 1 - b1 */
+  float beta2, rest2;         /* b2, 1 - b2 */
+  float step_size;            /* lr / (1 - b1^t) */
+  float inv_root_correction;  /* 1 / sqrt(1 - b2^t) */
+  float eps;
+  uint64_t philox_offset;
+} nvfp4_adamw_hyper;
+int nvfp4_adamw(const nvfp4_adamw_tensor* tensors, int count, const nvfp4_adamw_hyper* hypers, int n_hypers, int is_f32,
+                int state_bits, uint64_t philox_seed, const double* sumsq_parts, int n_parts, const float* norm,
+                float max_norm, float* norm_out, void* stream);
+
+/*
+ * Sum of the squares of many tensors (fp32, or bf16 when is_f32 == 0), in 64 bits, as nvfp4_sumsq_parts(count, counts)
+ * partial sums in `parts` (device), which nvfp4_adamw adds up in a fixed order, or nvfp4_norm_of_sumsq: *norm = their
+ * sum's root.  grads and counts are HOST arrays.  Parts of several calls may follow each other in one buffer.
+ */
+int nvfp4_sumsq_parts(int count, const int64_t* counts);   /* host arithmetic; negative = NVFP4_E_* */
+int nvfp4_sumsq(const void* const* grads, const int64_t* counts, int count, int is_f32, double* parts, void* stream);
+int nvfp4_norm_of_sumsq(const double* parts, int n_parts, float* norm, void* stream);
+
+/*
+ * Losses on logits [batch, seq, vocab] (fp32, or bf16 when is_f32 == 0; strides in elements, the logits of a row contiguous;
+ * rows are numbered batch * seq + position).  A row whose label equals ignore_index has no part in anything and is not read;
+ * any other label outside [0, vocab) gives NaN.  All row and sequence vectors are fp32.
+ */
+typedef struct {
+  const void* logits;
+  int is_f32;
+  int64_t batch, seq, vocab;
+  int64_t stride_b, stride_t;
+  const int64_t* labels;      /* [batch * seq] */
+  int64_t ignore_index;
+} nvfp4_logit_rows;           /* HOST struct, read before the call returns */
+/* Scratch of the calls that return a loss: device memory, 16-byte aligned, any content; calls that share it must not overlap. */
+#define NVFP4_LOSS_PARTS 1184
+#define NVFP4_LOSS_WORKSPACE (16 + 3 * 8 * NVFP4_LOSS_PARTS)
+
+/*
+ * logp[row] = x[label] - lse, lse[row] = log sum exp of the row (both 0 for an ignored row).
+ * Backward: dlogits (contiguous [batch, seq, vocab], the logits' type) = w (onehot(label) - exp(x - lse)), w =
+ * weight[row / rows_per_weight] (* *scale when given).  unless_one != 0: dlogits already holds the result for a scale of 1, and the
+ * call leaves it alone when *scale is 1.  The reference uses torch's cross_entropy (nvfp4_train.py:159-185).
+ */
+int nvfp4_logprob_fwd(const nvfp4_logit_rows* rows, float* logp, float* lse, void* stream);
+int nvfp4_logprob_bwd(const nvfp4_logit_rows* rows, const float* lse, const float* weight, int64_t rows_per_weight,
+                      const float* scale, int unless_one, void* dlogits, void* stream);
+
+/*
+ * Preference loss of batch / 2 pairs, sequence i chosen over sequence batch / 2 + i: with L_i the sum of the sequence's logp (fp64 here,
+ * [batch * seq]: a reward is a small difference of long sums),
+ * rewards[i] = beta (L_i - ref[i]), h = rewards[chosen] - rewards[rejected],
+ * loss = mean(-(1 - label_smoothing) logsigmoid(h) - label_smoothing logsigmoid(-h)).
+ * weight[i] = dloss / dL_i, for nvfp4_logprob_bwd with rows_per_weight = seq.  No counterpart in the reference.
+ */
+int nvfp4_preference_fwd(const nvfp4_logit_rows* rows, const float* ref, double beta, double label_smoothing, double* logp,
+                         float* lse, float* loss, float* rewards, float* weight, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/*
+ * Clipped policy loss with a KL term: rho = exp(logp - old_logp), A = advantage[row / rows_per_advantage], d = ref_logp - logp,
+ * loss = 1/n sum over the n rows with a label (n = 1 if there are none) of
+ *   -min(rho A, clamp(rho, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1)     (no KL term when ref_logp is NULL)
+ * stats2 = {mean of exp(d) - d - 1, share of rows whose clamp cut the gradient}; weight[row] = dloss / dlogp.
+ * dlogits: NULL, or the gradient of the loss for nvfp4_logprob_bwd's layout, written while the row is in L2.
+ * No counterpart in the reference.
+ */
+int nvfp4_policy_fwd(const nvfp4_logit_rows* rows, const float* old_logp, const float* advantage, int64_t rows_per_advantage,
+                     const float* ref_logp, double clip_low, double clip_high, double kl, float* logp, float* lse, float* weight,
+                     float* loss, float* stats2, void* dlogits, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Test hooks of the bounded waits, process-wide, for the launches that follow.  Every spin inside

@@ -1,18 +1,20 @@
-// Host side of the quantizer and GEMM entry points: argument handling, output allocation, stream lookup and the calls
-// into libnvfp4_b200.so, in C++.  quant.py and gemm.py keep the public functions, their defaults and the seed counter
-// and call in here.
+// Host side of the quantizer, GEMM and optimizer entry points: argument handling, output allocation, stream lookup and
+// the calls into libnvfp4_b200.so, in C++.  quant.py, gemm.py and optim.py keep the public functions, their defaults and
+// the seed counter and call in here.
 //
 // Why native: the small calls of this path are bound by the host.  One quantization took 25 us through Python (a
 // device context manager, three torch.empty, a ctypes call with sixteen arguments) for 6 us of kernel, an FP4Linear
 // step of 512 tokens 484 us for 74 us of kernels.
 #include <dlfcn.h>
 
+#include <cmath>
 #include <mutex>
 #include <unordered_map>
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "nvfp4_b200.h"
@@ -24,7 +26,8 @@ namespace {
 #define NVFP4_FOR_EACH(F)                                                                                              \
   F(nvfp4_amax_bf16) F(nvfp4_amax_both_bf16) F(nvfp4_quantize_fused_bf16) F(nvfp4_quantize_shard_bf16)                 \
   F(nvfp4_quantize_weight_bf16) F(nvfp4_quantize_dual_bf16) F(nvfp4_round_amax_f32) F(nvfp4_gemm) F(nvfp4_gemm_amax) \
-  F(nvfp4_gemm_bf16_as_f32)
+  F(nvfp4_gemm_bf16_as_f32) F(nvfp4_adamw) F(nvfp4_sumsq) F(nvfp4_sumsq_parts) F(nvfp4_norm_of_sumsq)       \
+  F(nvfp4_logprob_fwd) F(nvfp4_logprob_bwd) F(nvfp4_preference_fwd) F(nvfp4_policy_fwd)
 
 struct Library {
 #define F(name) decltype(&::name) name = nullptr;
@@ -343,6 +346,347 @@ at::Tensor mm_bf16_as_f32(const at::Tensor& aq, const at::Tensor& as, const at::
   return d;
 }
 
+// ---- optimizer ------------------------------------------------------------------------------------------------------
+const at::Tensor& tensor_of(PyObject* o) {
+  if (!THPVariable_Check(o)) raise(PyExc_TypeError, "expected a tensor");
+  return THPVariable_Unpack(o);
+}
+bool same_layout(const at::Tensor& a, const at::Tensor& b) {
+  if (a.sizes() != b.sizes()) return false;
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+// fp32 and bf16 tensors whose elements fill one piece of memory: the kernels go through it in its own order
+void check_param(const at::Tensor& p, c10::optional<c10::Device>& dev) {
+  if (!p.is_cuda() || (dev.has_value() && *dev != p.device())) {
+    const at::Tensor first = dev.has_value() ? at::empty({0}, on(*dev, at::kFloat)) : p;
+    device_of({&first, &p});                                // says what is wrong
+  }
+  dev = p.device();
+  if (p.scalar_type() != at::kFloat && p.scalar_type() != at::kBFloat16)
+    raise(PyExc_ValueError, std::string("parameters are fp32 or bf16, got ") + c10::toString(p.scalar_type()));
+  if (p.layout() != at::kStrided || !p.is_non_overlapping_and_dense())
+    raise(PyExc_ValueError, "parameters must fill their memory without gaps or overlaps");
+}
+// the gradient in the memory order of its parameter
+at::Tensor grad_like(const at::Tensor& p, const at::Tensor& g) {
+  if (g.layout() != at::kStrided) raise(PyExc_ValueError, "sparse gradients are not supported");
+  if (g.device() != p.device() || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes())
+    raise(PyExc_ValueError, "a gradient must have its parameter's device, dtype and shape");
+  if (same_layout(p, g) && !g.is_neg()) return g;
+  return at::empty_strided(p.sizes(), p.strides(), p.options().requires_grad(false)).copy_(g);
+}
+
+struct Grads {                                              // by dtype: bf16, fp32
+  std::vector<const void*> ptr[2];
+  std::vector<int64_t> n[2];
+  void add(const at::Tensor& g) {
+    const int k = g.scalar_type() == at::kFloat;
+    ptr[k].push_back(g.data_ptr());
+    n[k].push_back(g.numel());
+  }
+  // the partial sums of squares of all of them
+  at::Tensor parts(c10::Device dev) const {
+    int all = 0, some[2] = {0, 0};
+    for (int k = 0; k < 2; ++k) {
+      some[k] = lib.nvfp4_sumsq_parts((int)n[k].size(), n[k].data());
+      if (some[k] < 0) check(some[k], "nvfp4_sumsq_parts");
+      all += some[k];
+    }
+    at::Tensor parts = at::empty({all}, on(dev, at::kDouble));
+    double* at_ = static_cast<double*>(parts.data_ptr());
+    for (int k = 0; k < 2; ++k) {
+      if (n[k].empty()) continue;
+      check(lib.nvfp4_sumsq(ptr[k].data(), n[k].data(), (int)n[k].size(), k, at_, stream_of(dev)), "nvfp4_sumsq");
+      at_ += some[k];
+    }
+    return parts;
+  }
+};
+
+// Norm of the gradients of `params` (tensors that have none are skipped); None if none has one.
+py::object grad_norm(const py::list& params) {
+  Grads grads;
+  std::vector<at::Tensor> held;
+  c10::optional<c10::Device> dev;
+  for (py::handle h : params) {
+    const at::Tensor& p = tensor_of(h.ptr());
+    const at::Tensor& g = p.grad();
+    if (!g.defined() || g.numel() == 0) continue;
+    check_param(p, dev);
+    held.push_back(grad_like(p, g));
+    grads.add(held.back());
+  }
+  if (held.empty()) return py::none();
+  const c10::cuda::CUDAGuard guard(*dev);
+  const at::Tensor parts = grads.parts(*dev);
+  at::Tensor norm = at::empty({}, on(*dev, at::kFloat));
+  check(lib.nvfp4_norm_of_sumsq(static_cast<const double*>(parts.data_ptr()), (int)parts.numel(), float_ptr(norm),
+                                stream_of(*dev)),
+        "nvfp4_norm_of_sumsq");
+  return py::cast(norm);
+}
+
+PyObject* item(PyObject* dict, const char* key) {
+  PyObject* v = PyDict_GetItemString(dict, key);
+  if (v == nullptr) raise(PyExc_KeyError, key);
+  return v;
+}
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw py::error_already_set();
+  return v;
+}
+void check_state(const at::Tensor& t, c10::Device dev, at::ScalarType type, int64_t n, const char* name) {
+  if (t.device() != dev || t.scalar_type() != type || t.numel() != n)
+    raise(PyExc_ValueError, std::string("optimizer state '") + name + "' does not fit its parameter");
+}
+
+// One step of every parameter that has a gradient.  groups: the optimizer's param_groups; state: its state.  Returns False,
+// with nothing done, when a parameter has no state yet; None when no parameter has a gradient; else the norm of all
+// gradients (0-dim) if max_norm is given, or True.
+py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c10::optional<double> max_norm, uint64_t seed,
+                      const OptTensor& norm_in) {
+  struct Hyper {
+    double lr, b1, b2, eps, wd;
+  };
+  struct Item {
+    nvfp4_adamw_tensor t;
+    int group, f32;
+    int64_t step;
+    PyObject* state;
+  };
+  std::vector<Hyper> hypers;
+  std::vector<Item> items;
+  std::vector<at::Tensor> held;                              // gradients that had to be copied live until the launch
+  Grads grads;
+  c10::optional<c10::Device> dev;
+  uint64_t base = 0;
+  const bool eight = bits == 8;
+  for (py::handle gh : groups) {
+    PyObject* group = gh.ptr();
+    if (!PyDict_Check(group)) raise(PyExc_TypeError, "param_groups holds dicts");
+    const py::sequence betas = py::reinterpret_borrow<py::sequence>(item(group, "betas"));
+    hypers.push_back({number(item(group, "lr")), number(py::object(betas[0]).ptr()), number(py::object(betas[1]).ptr()),
+                      number(item(group, "eps")), number(item(group, "weight_decay"))});
+    for (py::handle ph : py::reinterpret_borrow<py::list>(item(group, "params"))) {
+      const at::Tensor& p = tensor_of(ph.ptr());
+      const int64_t n = p.numel(), blocks = (n + 255) / 256;
+      const uint64_t at_ = base;
+      base += (uint64_t)blocks * 32;                         // whether or not it has a gradient now
+      const at::Tensor& g0 = p.grad();
+      if (!g0.defined() || n == 0) continue;
+      check_param(p, dev);
+      at::Tensor g = grad_like(p, g0);
+      PyObject* st = PyDict_GetItemWithError(state.ptr(), ph.ptr());
+      if (st == nullptr) {
+        if (PyErr_Occurred()) throw py::error_already_set();
+        return py::bool_(false);
+      }
+      if (!PyDict_Check(st)) raise(PyExc_TypeError, "optimizer state holds dicts");
+      Item it{};
+      it.t.param = p.data_ptr();
+      it.t.grad = g.data_ptr();
+      it.t.n = n;
+      it.t.counter_base = at_;
+      it.group = (int)hypers.size() - 1;
+      it.f32 = p.scalar_type() == at::kFloat;
+      it.step = PyLong_AsLongLong(item(st, "step")) + 1;
+      if (it.step == 0 && PyErr_Occurred()) throw py::error_already_set();
+      it.state = st;
+      const at::Tensor& m = tensor_of(item(st, "exp_avg"));
+      const at::Tensor& v = tensor_of(item(st, eight ? "exp_avg_root" : "exp_avg_sq"));
+      if (eight) {
+        const at::Tensor& ms = tensor_of(item(st, "exp_avg_scale"));
+        const at::Tensor& vs = tensor_of(item(st, "exp_avg_root_scale"));
+        check_state(m, *dev, at::kFloat8_e4m3fn, blocks * 256, "exp_avg");
+        check_state(v, *dev, at::kFloat8_e4m3fn, blocks * 256, "exp_avg_root");
+        check_state(ms, *dev, at::kFloat8_e8m0fnu, blocks, "exp_avg_scale");
+        check_state(vs, *dev, at::kFloat8_e8m0fnu, blocks, "exp_avg_root_scale");
+        if (!m.is_contiguous() || !v.is_contiguous() || !ms.is_contiguous() || !vs.is_contiguous())
+          raise(PyExc_ValueError, "optimizer state must be contiguous");
+        it.t.first_scale = ms.data_ptr();
+        it.t.second_scale = vs.data_ptr();
+      } else {
+        check_state(m, *dev, at::kFloat, n, "exp_avg");
+        check_state(v, *dev, at::kFloat, n, "exp_avg_sq");
+        if (!same_layout(p, m) || !same_layout(p, v))
+          raise(PyExc_ValueError, "optimizer state must have its parameter's shape and strides");
+      }
+      it.t.first = m.data_ptr();
+      it.t.second = v.data_ptr();
+      grads.add(g);
+      if (!g.is_same(g0)) held.push_back(std::move(g));
+      items.push_back(it);
+    }
+  }
+  if (items.empty()) return py::none();
+  const c10::cuda::CUDAGuard guard(*dev);
+  at::Tensor parts, norm;
+  const double* parts_p = nullptr;
+  const float* norm_p = nullptr;
+  if (max_norm.has_value()) {
+    if (norm_in.has_value()) {
+      const at::Tensor anchor = at::empty({0}, on(*dev, at::kFloat));
+      device_of({&anchor, &*norm_in});
+      if (norm_in->scalar_type() != at::kFloat || norm_in->numel() != 1)
+        raise(PyExc_ValueError, "grad_norm must be one fp32 element");
+      norm = *norm_in;
+      norm_p = float_ptr(norm);
+    } else {
+      parts = grads.parts(*dev);
+      parts_p = static_cast<const double*>(parts.data_ptr());
+      norm = at::empty({}, on(*dev, at::kFloat));
+    }
+  }
+  // launches: one per dtype and up to eight different (group, step)
+  std::vector<nvfp4_adamw_tensor> ts;
+  std::vector<nvfp4_adamw_hyper> hs;
+  bool norm_out = parts_p != nullptr;
+  for (int f32 = 0; f32 < 2; ++f32) {
+    size_t i = 0;
+    while (i < items.size()) {
+      ts.clear();
+      hs.clear();
+      std::vector<std::pair<int, int64_t>> keys;
+      for (; i < items.size(); ++i) {
+        Item& it = items[i];
+        if (it.f32 != f32) continue;
+        const std::pair<int, int64_t> key{it.group, it.step};
+        size_t k = 0;
+        while (k < keys.size() && keys[k] != key) ++k;
+        if (k == keys.size()) {
+          if (k == 8) break;
+          keys.push_back(key);
+          const Hyper& h = hypers[it.group];
+          const double t = (double)it.step;
+          hs.push_back({(float)(1.0 - h.lr * h.wd), (float)h.b1, (float)(1.0 - h.b1), (float)h.b2, (float)(1.0 - h.b2),
+                        (float)(h.lr / (1.0 - std::pow(h.b1, t))), (float)(1.0 / std::sqrt(1.0 - std::pow(h.b2, t))),
+                        (float)h.eps, (uint64_t)it.step});
+        }
+        it.t.hyper = (int32_t)k;
+        ts.push_back(it.t);
+      }
+      if (ts.empty()) break;
+      check(lib.nvfp4_adamw(ts.data(), (int)ts.size(), hs.data(), (int)hs.size(), f32, bits, seed, parts_p,
+                            parts_p == nullptr ? 0 : (int)parts.numel(), norm_p, max_norm.value_or(0.0),
+                            norm_out ? float_ptr(norm) : nullptr, stream_of(*dev)),
+            "nvfp4_adamw");
+      norm_out = false;
+    }
+  }
+  for (const Item& it : items) {
+    const py::int_ step(it.step);
+    if (PyDict_SetItemString(it.state, "step", step.ptr()) != 0) throw py::error_already_set();
+  }
+  // the parameters changed in place, as any optimizer changes them
+  for (py::handle gh : groups)
+    for (py::handle ph : py::reinterpret_borrow<py::list>(item(gh.ptr(), "params"))) {
+      const at::Tensor& p = tensor_of(ph.ptr());
+      if (p.grad().defined()) p.unsafeGetTensorImpl()->bump_version();
+    }
+  if (norm.defined()) return py::cast(norm);
+  return py::bool_(true);
+}
+
+// ---- losses on logits -----------------------------------------------------------------------------------------------
+// Logits [rows, vocab] or [batch, seq, vocab] and their labels as the kernels read them.
+struct Logits {
+  at::Tensor x, labels;                                     // x is the caller's tensor wherever the kernels can read that
+  nvfp4_logit_rows rows;
+  c10::Device dev{c10::kCUDA};
+  Logits(const at::Tensor& logits, const at::Tensor& labels_in, int64_t ignore) {
+    if (logits.dim() != 2 && logits.dim() != 3) raise(PyExc_ValueError, "logits must be [rows, vocab] or [batch, seq, vocab]");
+    if (labels_in.sizes() != logits.sizes().slice(0, logits.dim() - 1))
+      raise(PyExc_ValueError, "labels must have the shape of the logits without the last dimension");
+    if (logits.scalar_type() != at::kFloat && logits.scalar_type() != at::kBFloat16)
+      raise(PyExc_ValueError, std::string("logits are fp32 or bf16, got ") + c10::toString(logits.scalar_type()));
+    if (!c10::isIntegralType(labels_in.scalar_type(), false)) raise(PyExc_ValueError, "labels must be integers");
+    if (logits.numel() == 0) raise(PyExc_ValueError, "logits are empty");
+    dev = device_of({&logits, &labels_in});
+    x = logits.resolve_neg();
+    if (x.stride(-1) != 1 && x.size(-1) > 1) x = x.contiguous();
+    labels = labels_in.to(at::kLong).contiguous();
+    const bool three = x.dim() == 3;
+    rows = nvfp4_logit_rows{x.data_ptr(), x.scalar_type() == at::kFloat, three ? x.size(0) : 1, x.size(-2), x.size(-1),
+                            three ? x.stride(0) : 0, x.stride(-2), labels.data_ptr<int64_t>(), ignore};
+  }
+  int64_t count() const { return rows.batch * rows.seq; }
+  at::Tensor per_row() const { return at::empty(labels.sizes(), on(dev, at::kFloat)); }
+  // a row or sequence vector as the kernels read it
+  at::Tensor vec(const at::Tensor& t, int64_t n, const char* name) const {
+    device_of({&x, &t});
+    if (t.numel() != n || !t.is_floating_point()) raise(PyExc_ValueError, std::string(name) + " must hold " + std::to_string(n) + " floating-point values");
+    return t.to(at::kFloat).contiguous();
+  }
+};
+
+py::tuple logprob_fwd(const at::Tensor& logits, const at::Tensor& labels, int64_t ignore) {
+  const Logits in(logits, labels, ignore);
+  const c10::cuda::CUDAGuard guard(in.dev);
+  at::Tensor logp = in.per_row(), lse = in.per_row();
+  check(lib.nvfp4_logprob_fwd(&in.rows, float_ptr(logp), float_ptr(lse), stream_of(in.dev)), "nvfp4_logprob_fwd");
+  return py::make_tuple(logp, lse);
+}
+
+// weight: dloss / dlogp, one per row or one per sequence; scale: what it is to be multiplied with (one element); ready: the
+// gradient for a scale of 1, to be used again where the scale is 1
+at::Tensor logprob_bwd(const at::Tensor& logits, const at::Tensor& labels, int64_t ignore, const at::Tensor& lse,
+                       const at::Tensor& weight, const OptTensor& scale, const OptTensor& ready) {
+  const Logits in(logits, labels, ignore);
+  const c10::cuda::CUDAGuard guard(in.dev);
+  const at::Tensor w = in.vec(weight, weight.numel() == in.rows.batch ? in.rows.batch : in.count(), "weight");
+  at::Tensor sc;
+  if (scale.has_value()) sc = in.vec(*scale, 1, "scale");
+  at::Tensor out = ready.has_value() ? *ready : at::empty(logits.sizes(), on(in.dev, logits.scalar_type()));
+  check(lib.nvfp4_logprob_bwd(&in.rows, float_ptr(lse), float_ptr(w), in.count() / w.numel(), sc.defined() ? float_ptr(sc) : nullptr,
+                              ready.has_value(), out.data_ptr(), stream_of(in.dev)),
+        "nvfp4_logprob_bwd");
+  return out;
+}
+
+at::Tensor loss_workspace(c10::Device dev) { return at::empty({NVFP4_LOSS_WORKSPACE}, on(dev, at::kByte)); }
+
+// (loss, rewards, lse, weight)
+py::tuple preference_fwd(const at::Tensor& logits, const at::Tensor& labels, int64_t ignore, const at::Tensor& ref, double beta,
+                         double smoothing) {
+  const Logits in(logits, labels, ignore);
+  const c10::cuda::CUDAGuard guard(in.dev);
+  if (logits.dim() != 3 || in.rows.batch % 2 != 0)
+    raise(PyExc_ValueError, "logits must be [2 pairs, seq, vocab], the chosen sequences first");
+  const at::Tensor r = in.vec(ref, in.rows.batch, "ref_logps");
+  at::Tensor logp = at::empty({in.count()}, on(in.dev, at::kDouble)), lse = in.per_row(), loss = at::empty({}, on(in.dev, at::kFloat)),
+             rewards = at::empty({in.rows.batch}, on(in.dev, at::kFloat)), weight = at::empty_like(rewards);
+  const at::Tensor ws = loss_workspace(in.dev);
+  check(lib.nvfp4_preference_fwd(&in.rows, float_ptr(r), beta, smoothing, static_cast<double*>(logp.data_ptr()), float_ptr(lse), float_ptr(loss),
+                                 float_ptr(rewards), float_ptr(weight), ws.data_ptr(), ws.numel(), stream_of(in.dev)),
+        "nvfp4_preference_fwd");
+  return py::make_tuple(loss, rewards, lse, weight);
+}
+
+// (loss, stats, logp, lse, weight, gradient of the logits or None)
+py::tuple policy_fwd(const at::Tensor& logits, const at::Tensor& labels, int64_t ignore, const at::Tensor& old_logps,
+                     const at::Tensor& advantages, const OptTensor& ref, double low, double high, double kl, bool want_grad) {
+  const Logits in(logits, labels, ignore);
+  const c10::cuda::CUDAGuard guard(in.dev);
+  const int64_t n = in.count();
+  const bool per_sequence = advantages.dim() == 1 && logits.dim() == 3;
+  const at::Tensor old = in.vec(old_logps, n, "old_logps"),
+                   adv = in.vec(advantages, per_sequence ? in.rows.batch : n, "advantages");
+  at::Tensor rf, grad;
+  if (ref.has_value()) rf = in.vec(*ref, n, "ref_logps");
+  at::Tensor logp = in.per_row(), lse = in.per_row(), weight = in.per_row(), loss = at::empty({}, on(in.dev, at::kFloat)),
+             stats = at::empty({2}, on(in.dev, at::kFloat));
+  if (want_grad) grad = at::empty(logits.sizes(), on(in.dev, logits.scalar_type()));
+  const at::Tensor ws = loss_workspace(in.dev);
+  check(lib.nvfp4_policy_fwd(&in.rows, float_ptr(old), float_ptr(adv), n / adv.numel(), rf.defined() ? float_ptr(rf) : nullptr, low,
+                             high, kl, float_ptr(logp), float_ptr(lse), float_ptr(weight), float_ptr(loss), float_ptr(stats),
+                             want_grad ? grad.data_ptr() : nullptr, ws.data_ptr(), ws.numel(), stream_of(in.dev)),
+        "nvfp4_policy_fwd");
+  return py::make_tuple(loss, stats, logp, lse, weight, want_grad ? py::cast(grad) : py::none());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -357,4 +701,10 @@ PYBIND11_MODULE(_host, m) {
   m.def("quantize_dual", &quantize_dual);
   m.def("mm", &mm);
   m.def("mm_bf16_as_f32", &mm_bf16_as_f32);
+  m.def("grad_norm", &grad_norm);
+  m.def("adamw_step", &adamw_step);
+  m.def("logprob_fwd", &logprob_fwd);
+  m.def("logprob_bwd", &logprob_bwd);
+  m.def("preference_fwd", &preference_fwd);
+  m.def("policy_fwd", &policy_fwd);
 }

@@ -20,6 +20,8 @@
 // ones a thread: 32-byte accesses, and one warp is one 256-element block, whose maximum is one redux per moment.
 #include <type_traits>
 
+#include <cuda_fp16.h>
+
 #include "quantize_common.cuh"
 
 namespace nvfp4 {
@@ -42,8 +44,8 @@ struct Entry {
   int32_t hyper;
   int32_t wide;              // every pointer takes 32-byte (16-byte for bf16) accesses
 };
-struct Hyper {
-  float decay, beta1, rest1, beta2, rest2, step, inv_root, eps;
+struct Hyper {               // each twice, as the packed instructions take them: one load from constant memory, no copies
+  float2 decay, beta1, rest1, beta2, rest2, step, inv_root, eps, one;       // step: with its sign
   uint64_t offset;
 };
 template <int CAP> struct Table {
@@ -60,8 +62,8 @@ struct Clip {
   float* norm_out;           // the norm that was used
 };
 
-// the tensor that chunk c belongs to
-template <int CAP> __device__ __forceinline__ int find(const Table<CAP>& t, uint32_t c) {
+// The tensor that chunk c belongs to.
+template <class Table> __device__ __forceinline__ int find(const Table& t, uint32_t c) {
   int lo = 0, hi = t.count;                      // start[lo] <= c < start[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -71,47 +73,73 @@ template <int CAP> __device__ __forceinline__ int find(const Table<CAP>& t, uint
   return lo;
 }
 
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  asm("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(p) : "memory");
+// Pairs of fp32 in the two lanes of sm_100's packed instructions.
+struct Eight {
+  float2 v[4];
+  __device__ __forceinline__ float& operator[](int j) { return j & 1 ? v[j >> 1].y : v[j >> 1].x; }
+};
+// Eight elements as they lie in memory.  They are opened where they are used: a conversion behind the load would wait for
+// that load in front of the next one.
+template <class T> struct Raw;
+template <> struct Raw<float> {
+  float w[8];
+  __device__ __forceinline__ void load(const float* p) {
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3]), "=f"(w[4]), "=f"(w[5]), "=f"(w[6]), "=f"(w[7]) : "l"(p) : "memory");
+  }
+  __device__ __forceinline__ void gather(const float* p, int64_t left) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = j < left ? p[j] : 0.0f;
+  }
+  __device__ __forceinline__ Eight open() const {
+    return Eight{{make_float2(w[0], w[1]), make_float2(w[2], w[3]), make_float2(w[4], w[5]), make_float2(w[6], w[7])}};
+  }
+};
+template <> struct Raw<__nv_bfloat16> {
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p) : "memory");
+  }
+  __device__ __forceinline__ void gather(const __nv_bfloat16* p, int64_t left) {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = (2 * j < left ? (uint32_t)h[2 * j] : 0u) | (2 * j + 1 < left ? (uint32_t)h[2 * j + 1] << 16 : 0u);
+  }
+  __device__ __forceinline__ Eight open() const {
+    Eight x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x.v[j] = make_float2(bf16_lo(w[j]), bf16_hi(w[j]));
+    return x;
+  }
+};
+// eight elements from `at` on, those behind the end as zeros
+template <class T> __device__ __forceinline__ void fetch(const T* p, int64_t at, int64_t n, bool whole, Raw<T>& x) {
+  if (whole) x.load(p + at);
+  else x.gather(p + at, n - at);
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 q = *reinterpret_cast<const uint4*>(p);
-  v[0] = bf16_lo(q.x); v[1] = bf16_hi(q.x); v[2] = bf16_lo(q.y); v[3] = bf16_hi(q.y);
-  v[4] = bf16_lo(q.z); v[5] = bf16_hi(q.z); v[6] = bf16_lo(q.w); v[7] = bf16_hi(q.w);
-}
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+
+__device__ __forceinline__ void store8(float* p, const Eight& x) {
   asm volatile("st.global.v8.f32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
-      :: "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "l"(p) : "memory");
+      :: "f"(x.v[0].x), "f"(x.v[0].y), "f"(x.v[1].x), "f"(x.v[1].y), "f"(x.v[2].x), "f"(x.v[2].y), "f"(x.v[3].x),
+         "f"(x.v[3].y), "l"(p) : "memory");
 }
-__device__ __forceinline__ uint32_t pack(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+__device__ __forceinline__ uint32_t pack(float2 a) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a.x, a.y);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7]));
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const Eight& x) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack(x.v[0]), pack(x.v[1]), pack(x.v[2]), pack(x.v[3]));
 }
-__device__ __forceinline__ float as_float(float v) { return v; }
-__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
-// eight elements from `at` on, those behind the end as zeros
-template <class T> __device__ __forceinline__ void fetch(const T* p, int64_t at, int64_t n, bool whole, float (&v)[8]) {
+template <class T> __device__ __forceinline__ void keep(T* p, int64_t at, int64_t n, bool whole, Eight& x) {
   if (whole) {
-    load8(p + at, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = at + j < n ? as_float(p[at + j]) : 0.0f;
-  }
-}
-template <class T> __device__ __forceinline__ void keep(T* p, int64_t at, int64_t n, bool whole, const float (&v)[8]) {
-  if (whole) {
-    store8(p + at, v);
+    store8(p + at, x);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (at + j < n) put(p + at + j, v[j]);
+      if (at + j < n) put(p + at + j, x[j]);
   }
 }
 
@@ -130,7 +158,7 @@ __device__ __forceinline__ double cta_sum(double s) {
   return s;
 }
 
-constexpr int kNormCap = 512;
+constexpr int kNormCap = 512, kNormGrid = 148 * 4;
 struct NormTable {
   const void* grad[kNormCap];
   int64_t n[kNormCap];
@@ -139,24 +167,29 @@ struct NormTable {
   int32_t count;
 };
 
+constexpr int kNormChunk = 4 * kChunk;             // four loads of eight elements in flight in each thread
 template <class T>
 __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ NormTable t, double* __restrict__ parts) {
   double sum = 0.0;
   const uint32_t total = t.start[t.count];
-  for (uint32_t c = blockIdx.x; c < total; c += gridDim.x) {
-    int lo = 0, hi = t.count;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (t.start[mid] <= c) lo = mid;
-      else hi = mid;
-    }
-    const T* g = static_cast<const T*>(t.grad[lo]);
-    const int64_t n = t.n[lo], at = (int64_t)(c - t.start[lo]) * kChunk + threadIdx.x * 8;
-    if (at >= n) continue;
-    float v[8];
-    fetch(g, at, n, t.wide[lo] && at + 8 <= n, v);
+  uint32_t c = blockIdx.x;
+  int k = c < total ? find(t, c) : 0;
+  for (; c < total; c += gridDim.x) {
+    while (t.start[k + 1] <= c) ++k;
+    const T* g = static_cast<const T*>(t.grad[k]);
+    const int64_t n = t.n[k], at = (int64_t)(c - t.start[k]) * kNormChunk + threadIdx.x * 8;
+    const bool wide = t.wide[k];
+    Raw<T> x[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum = fma((double)v[j], (double)v[j], sum);
+    for (int u = 0; u < 4; ++u)
+      if (at + u * kChunk < n) fetch(g, at + u * kChunk, n, wide && at + u * kChunk + 8 <= n, x[u]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (at + u * kChunk < n) {
+        Eight v = x[u].open();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fma((double)v[j], (double)v[j], sum);
+      }
   }
   sum = cta_sum(sum);
   if (threadIdx.x == 0) parts[blockIdx.x] = sum;
@@ -173,123 +206,244 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict
 }
 
 // ---- the step --------------------------------------------------------------------------------------------------------
-// E4M3 codes of eight elements -> fp32; f = 2^(e + 49).  The code's exponent and mantissa in bits 20 to 26 make an fp32
-// (or a denormal) 2^120 too small; both products are exact.
-__device__ __forceinline__ void decode8(uint2 q, uint8_t scale, float (&v)[8]) {
-  const float f = scale == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(min((uint32_t)scale + 56u, 254u) << 23);
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+// a + b as a * 1 + b with a 1 that the compiler does not see: nvcc 12.9 and its assembler make one fused multiply-add of a
+// packed product and a packed sum, roundings asked for or not
+__device__ __forceinline__ float2 add2(float2 a, float2 b, float2 one) { return __ffma2_rn(a, one, b); }
+// max(|a|, |b|, |c|), a NaN if one of them is
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  return r;
+}
+
+// Eight E4M3 codes under an E8M0 scale -> fp32 (every product is exact).
+__device__ __forceinline__ void decode8(uint2 q, uint32_t scale, Eight& x) {
+  const uint32_t f = scale == 255u ? 0x7fc00000u : scale == 0u ? 0x00400000u : scale << 23;
+  const float2 ff = both(__uint_as_float(f));
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t b = (j < 4 ? q.x : q.y) >> (8 * (j & 3));
-    v[j] = (__uint_as_float(((b & 0x80u) << 24) | ((b & 0x7fu) << 20)) * 0x1p64f) * f;
+  for (int j = 0; j < 4; ++j) {
+    const uint16_t two = (uint16_t)((j < 2 ? q.x : q.y) >> (16 * (j & 1)));
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
+    x.v[j] = mul2(__half22float2(*reinterpret_cast<const __half2*>(&h)), ff);
   }
 }
 
-// Codes of eight elements under the block's scale, which lane 0 stores; d: 16 random bits each.
-__device__ __forceinline__ uint2 encode8(const float (&v)[8], const uint32_t (&d)[8], uint8_t* scale, bool live) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-  top = __reduce_max_sync(0xffffffffu, top);
+// Codes of eight elements under the block's scale, which lane 0 stores; d: words of 16 random bits for each.
+template <bool SIGNED> __device__ __forceinline__ uint2 encode8(Eight x, const uint32_t (&d)[8], uint8_t* scale) {
+  const float top_f = max3_abs_nan(max3_abs_nan(x[0], x[1], x[2]), x[3], x[4]);
+  const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(max3_abs_nan(max3_abs_nan(top_f, x[5], x[6]), x[7], x[7])));
   const uint32_t e = min(max(top >> 23, 27u), 177u);
   // a block with an element of 2^51 or more, an infinity or a NaN is held as NaN
-  if (live && (threadIdx.x & 31) == 0) *scale = (top >> 23) > 177u ? 255 : (uint8_t)(e - 7);
-  const float h = __uint_as_float((205u - e) << 23);
-  uint32_t w[2] = {0u, 0u};
+  if ((threadIdx.x & 31) == 0) *scale = (top >> 23) > 177u ? 255 : (uint8_t)(e - 7);
+  float2 h = both(__uint_as_float((141u - e) << 23));       // 2^-(113 + its exponent)
+  if (e > 140u) {                                            // below fp32's normal numbers: in two steps
+    h = both(__uint_as_float((205u - e) << 23));
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float y = (fabsf(v[j]) * h) * 0x1p-64f;
-    const uint32_t code = ((__float_as_uint(y) + (d[j] << 4)) >> 20) & 0x7fu;
-    w[j >> 2] |= (code | ((__float_as_uint(v[j]) >> 24) & 0x80u)) << (8 * (j & 3));
+    for (int j = 0; j < 4; ++j) x.v[j] = mul2(x.v[j], both(0x1p-64f));
   }
-  return make_uint2(w[0], w[1]);
+  uint32_t u[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 y = mul2(x.v[j], h);
+    u[2 * j] = __float_as_uint(y.x) + (d[2 * j] << 4);       // (the sign bit stays: the magnitude ends at bit 26)
+    u[2 * j + 1] = __float_as_uint(y.y) + (d[2 * j + 1] << 4);
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t tops = __byte_perm(u[2 * j], u[2 * j + 1], 0x7632);       // sign, four zeros, code, four bits below it; twice
+    w[j] = tops >> 4;
+    if (SIGNED) w[j] = (w[j] & 0x007f007fu) | ((tops >> 8) & 0xff80ff80u);
+  }
+  return make_uint2(__byte_perm(w[0], w[1], 0x6420), __byte_perm(w[2], w[3], 0x6420));
 }
 
-template <class T, bool EIGHT, int CAP>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<CAP> t, const Clip clip,
-                                                         const PhiloxKeys keys) {
-  float c = 1.0f;
-  const bool clipped = clip.parts != nullptr || clip.norm != nullptr;
-  if (clipped) {
-    const float norm = clip.parts != nullptr ? norm_of(clip.parts, clip.n_parts) : *clip.norm;
-    if (blockIdx.x == 0 && threadIdx.x == 0 && clip.norm_out != nullptr) *clip.norm_out = norm;
-    c = __fdiv_rn(clip.max_norm, __fadd_rn(norm, 1e-6f));
-    c = c > 1.0f ? 1.0f : c;                     // (a NaN stays one)
-  }
-  const int64_t total = t.start[t.count];
-  for (int64_t chunk = total - 1 - blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
-    const int k = find(t, (uint32_t)chunk);
+// c = min(1, max_norm / (norm + 1e-6)), 1 without clipping; the first CTA leaves the norm for the caller.
+__device__ __forceinline__ float clip_factor(const Clip& clip) {
+  if (clip.parts == nullptr && clip.norm == nullptr) return 1.0f;
+  const float norm = clip.parts != nullptr ? norm_of(clip.parts, clip.n_parts) : *clip.norm;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && clip.norm_out != nullptr) *clip.norm_out = norm;
+  const float c = __fdiv_rn(clip.max_norm, __fadd_rn(norm, 1e-6f));
+  return c > 1.0f ? 1.0f : c;                    // (a NaN stays one)
+}
+
+// Both kernels go through the chunks last one first: the norm's pass has just read the gradients in their order, and the last
+// of them are still in L2.
+template <class T, int CAP>
+__global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constant__ Table<CAP> t, const Clip clip) {
+  const float c = clip_factor(clip);
+  int64_t chunk = (int64_t)t.start[t.count] - 1 - blockIdx.x;
+  if (chunk < 0) return;
+  int k = find(t, (uint32_t)chunk);
+  for (; chunk >= 0; chunk -= gridDim.x) {
+    while (t.start[k] > (uint32_t)chunk) --k;
     const Entry& e = t.e[k];
     const Hyper& h = t.h[e.hyper];
     const int64_t n = e.n, at = (chunk - t.start[k]) * kChunk + threadIdx.x * 8;
+    if (at >= n) continue;
     const bool whole = e.wide && at + 8 <= n;
-    T* param = static_cast<T*>(e.param);
-    float p[8], g[8], m[8], r[8];
-    if (EIGHT) {
-      // the warp's block; lanes behind the end of the tensor but inside the block carry zeros, other warps nothing
-      if ((at & ~(int64_t)(kBlock - 1)) >= n) continue;
-      decode8(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(e.first) + at), e.first_scale[at / kBlock], m);
-      decode8(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(e.second) + at), e.second_scale[at / kBlock], r);
-      fetch(param, at, n, whole, p);
-      fetch(static_cast<const T*>(e.grad), at, n, whole, g);
+    Raw<T> param, grad;
+    Raw<float> first, second;
+    fetch(static_cast<const T*>(e.param), at, n, whole, param);
+    fetch(static_cast<const T*>(e.grad), at, n, whole, grad);
+    fetch(static_cast<const float*>(e.first), at, n, whole, first);
+    fetch(static_cast<const float*>(e.second), at, n, whole, second);
+    Eight p = param.open(), g = grad.open(), m = first.open(), v = second.open();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = __fmul_rn(r[j], r[j]);
-    } else {
-      if (at >= n) continue;
-      fetch(param, at, n, whole, p);
-      fetch(static_cast<const T*>(e.grad), at, n, whole, g);
-      fetch(static_cast<const float*>(e.first), at, n, whole, m);
-      fetch(static_cast<const float*>(e.second), at, n, whole, r);
+    for (int j = 0; j < 4; ++j) {
+      const float2 gg = mul2(g.v[j], both(c));               // (by 1 when nothing is clipped)
+      m.v[j] = add2(mul2(m.v[j], h.beta1), mul2(gg, h.rest1), h.one);
+      v.v[j] = add2(mul2(v.v[j], h.beta2), mul2(mul2(gg, h.rest2), gg), h.one);
     }
+    keep(static_cast<float*>(e.first), at, n, whole, m);
+    keep(static_cast<float*>(e.second), at, n, whole, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (clipped) g[j] = __fmul_rn(g[j], c);
-      m[j] = __fadd_rn(__fmul_rn(m[j], h.beta1), __fmul_rn(g[j], h.rest1));
-      r[j] = __fadd_rn(__fmul_rn(r[j], h.beta2), __fmul_rn(__fmul_rn(g[j], h.rest2), g[j]));
+    for (int j = 0; j < 4; ++j) {
+      const float2 root = make_float2(__fsqrt_rn(v.v[j].x), __fsqrt_rn(v.v[j].y));
+      const float2 below = add2(mul2(root, h.inv_root), h.eps, h.one);
+      const float2 ratio = make_float2(__fdiv_rn(m.v[j].x, below.x), __fdiv_rn(m.v[j].y, below.y));
+      p.v[j] = add2(mul2(p.v[j], h.decay), mul2(ratio, h.step), h.one);
     }
-    if (!EIGHT) {
-      keep(static_cast<float*>(e.first), at, n, whole, m);
-      keep(static_cast<float*>(e.second), at, n, whole, r);
-    }
+    keep(static_cast<T*>(e.param), at, n, whole, p);
+  }
+}
+
+__device__ __forceinline__ float root_approx(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The same step on 8-bit moments.  It is bound by instructions as much as by memory (75 for an element with the arithmetic
+// above, 16 or 10 bytes), so here products are fused with their sums and root and quotient are the approximate
+// instructions: 2^-22 of an update, beside moments that hold 2^-4.
+//
+// A warp takes two blocks in a row of fp32 parameters, four of bf16, with the loads of all of them in flight before the
+// first is worked on; the table, the constants and the addresses are worked out once for them.  Two CTAs of 128 registers
+// a thread then beat three or four of fewer (124M fp32 parameters 355 us, 409 with one block and three CTAs, 411 with one and
+// four; 222M bf16 ones 459, 564, 533), and copying ahead to shared memory (353 to 514, 576 to 597).
+template <class T> constexpr int kRun = 8 / sizeof(T);
+template <class T> constexpr int kChunk8 = kRun<T> * kChunk;
+template <class T> struct Item8 {
+  Raw<T> param, grad;
+  uint2 first, second;
+  uint32_t first_scale, second_scale;
+};
+// The step of one block: x in; p, the codes and the scales (at `first_scale` and `second_scale`) out.  left: elements from this
+// thread's first to the end of the tensor.
+template <class T>
+__device__ __forceinline__ void step8(const Item8<T>& x, const Hyper& h, float c, const PhiloxKeys& keys, uint64_t group, int64_t left,
+                                      Eight& p, uint8_t* first, uint8_t* second, uint8_t* first_scale, uint8_t* second_scale) {
+  Eight m, r;
+  p = x.param.open();
+  const Eight g8 = x.grad.open();
+  decode8(x.first, x.first_scale, m);
+  decode8(x.second, x.second_scale, r);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      r[j] = __fsqrt_rn(r[j]);
-      const float ratio = __fdiv_rn(m[j], __fadd_rn(__fmul_rn(r[j], h.inv_root), h.eps));
-      p[j] = __fsub_rn(__fmul_rn(p[j], h.decay), __fmul_rn(ratio, h.step));
-    }
-    keep(param, at, n, whole, p);
-    if (EIGHT) {
+  for (int j = 0; j < 4; ++j) {
+    const float2 g = __fmul2_rn(g8.v[j], both(c));
+    m.v[j] = __ffma2_rn(m.v[j], h.beta1, __fmul2_rn(g, h.rest1));
+    const float2 v = __ffma2_rn(__fmul2_rn(r.v[j], r.v[j]), h.beta2, __fmul2_rn(__fmul2_rn(g, h.rest2), g));
+    r.v[j] = make_float2(root_approx(v.x), root_approx(v.y));
+    const float2 below = __ffma2_rn(r.v[j], h.inv_root, h.eps);
+    const float2 ratio = __fmul2_rn(m.v[j], make_float2(reciprocal_approx(below.x), reciprocal_approx(below.y)));
+    p.v[j] = __ffma2_rn(ratio, h.step, __fmul2_rn(p.v[j], h.decay));
+  }
+  if (left < 8) {                                            // (eps 0 or a NaN factor must not reach the block's scale from there)
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (at + j >= n) m[j] = r[j] = 0.0f;     // (eps 0 or a NaN factor must not reach the block's scale from there)
-      const uint64_t group = e.group + (uint64_t)at / 8;
-      const Philox4 x = fused::philox_rounds((uint32_t)group, (uint32_t)(group >> 32), (uint32_t)h.offset,
-                                             (uint32_t)(h.offset >> 32), keys);
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-      uint32_t d[8], b[8];
+    for (int j = 0; j < 8; ++j)
+      if (j >= left) m[j] = r[j] = 0.0f;
+  }
+  const Philox4 y = fused::philox_rounds((uint32_t)group, (uint32_t)(group >> 32), (uint32_t)h.offset,
+                                         (uint32_t)(h.offset >> 32), keys);
+  const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+  uint32_t d[8], b[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t turned = __brev(w[j]);
-        d[2 * j] = w[j] & 0xffffu; d[2 * j + 1] = w[j] >> 16;
-        b[2 * j] = turned >> 16; b[2 * j + 1] = turned & 0xffffu;
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t turned = __brev(w[j]);
+    d[2 * j] = w[j] & 0xffffu; d[2 * j + 1] = w[j] >> 16;
+    b[2 * j] = turned >> 16; b[2 * j + 1] = turned & 0xffffu;
+  }
+  *reinterpret_cast<uint2*>(first) = encode8<true>(m, d, first_scale);
+  *reinterpret_cast<uint2*>(second) = encode8<false>(r, b, second_scale);
+}
+
+constexpr int kResident8 = 2;
+template <class T, int CAP>
+__global__ void __launch_bounds__(kThreads, kResident8) adamw8_kernel(const __grid_constant__ Table<CAP> t, const Clip clip,
+                                                                      const PhiloxKeys keys) {
+  const float c = clip_factor(clip);
+  int64_t chunk = (int64_t)t.start[t.count] - 1 - blockIdx.x;
+  if (chunk < 0) return;
+  int k = find(t, (uint32_t)chunk);
+  for (; chunk >= 0; chunk -= gridDim.x) {
+    while (t.start[k] > (uint32_t)chunk) --k;
+    const Entry& e = t.e[k];
+    const Hyper& h = t.h[e.hyper];
+    const int64_t n = e.n, run = (chunk - t.start[k]) * kChunk8<T> + (threadIdx.x >> 5) * (kRun<T> * kBlock);
+    const int64_t at = run + (threadIdx.x & 31) * 8;
+    if (run >= n) continue;
+    T* param = static_cast<T*>(e.param) + at;
+    const T* grad = static_cast<const T*>(e.grad) + at;
+    uint8_t *first = static_cast<uint8_t*>(e.first) + at, *second = static_cast<uint8_t*>(e.second) + at;
+    uint8_t *first_scale = e.first_scale + run / kBlock, *second_scale = e.second_scale + run / kBlock;
+    const uint64_t group = e.group + (uint64_t)at / 8;
+    Eight p;
+    if (e.wide && run + kRun<T> * kBlock <= n) {
+      Item8<T> x[kRun<T>];
+#pragma unroll
+      for (int u = 0; u < kRun<T>; ++u) {
+        x[u].first = *reinterpret_cast<const uint2*>(first + u * kBlock);
+        x[u].second = *reinterpret_cast<const uint2*>(second + u * kBlock);
+        x[u].first_scale = first_scale[u];
+        x[u].second_scale = second_scale[u];
+        x[u].param.load(param + u * kBlock);
+        x[u].grad.load(grad + u * kBlock);
       }
-      const uint2 qm = encode8(m, d, e.first_scale + at / kBlock, true);
-      const uint2 qr = encode8(r, b, e.second_scale + at / kBlock, true);
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(e.first) + at) = qm;
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(e.second) + at) = qr;
+#pragma unroll
+      for (int u = 0; u < kRun<T>; ++u) {
+        step8<T>(x[u], h, c, keys, group + u * (kBlock / 8), 8, p, first + u * kBlock, second + u * kBlock, first_scale + u,
+                 second_scale + u);
+        store8(param + u * kBlock, p);
+      }
+    } else {                                                 // a run that ends in it, or one that lies off the vectors' boundaries
+#pragma unroll 1
+      for (int u = 0; u < kRun<T> && run + u * kBlock < n; ++u) {
+        const int64_t left = n - at - u * kBlock;            // lanes behind the end but inside the block carry zeros
+        const bool whole = e.wide && left >= 8;
+        Item8<T> x;
+        fetch(param + u * kBlock, 0, left, whole, x.param);
+        fetch(grad + u * kBlock, 0, left, whole, x.grad);
+        x.first = *reinterpret_cast<const uint2*>(first + u * kBlock);
+        x.second = *reinterpret_cast<const uint2*>(second + u * kBlock);
+        x.first_scale = first_scale[u];
+        x.second_scale = second_scale[u];
+        step8<T>(x, h, c, keys, group + u * (kBlock / 8), left, p, first + u * kBlock, second + u * kBlock, first_scale + u,
+                 second_scale + u);
+        keep(param + u * kBlock, 0, left, whole, p);
+      }
     }
   }
 }
 
 template <int CAP> constexpr bool fits() { return sizeof(Table<CAP>) + sizeof(Clip) + sizeof(PhiloxKeys) <= 32764; }
-constexpr int kSmall = 48, kLarge = 400;
+constexpr int kSmall = 64, kLarge = 400;
 static_assert(fits<kLarge>() && sizeof(NormTable) + 8 <= 32764, "kernel parameters are 32764 bytes at most");
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 template <class T, bool EIGHT, int CAP>
-int launch(const nvfp4_adamw_tensor* ts, int count, const nvfp4_adamw_hyper* hs, int n_hypers, const Clip& clip,
+int launch_step(const nvfp4_adamw_tensor* ts, int count, const nvfp4_adamw_hyper* hs, int n_hypers, const Clip& clip,
            const PhiloxKeys& keys, cudaStream_t stream) {
-  static_assert(sizeof(T) == 2 || sizeof(T) == 4, "");
+  constexpr int chunk = EIGHT ? kChunk8<T> : kChunk, resident = 148 * (EIGHT ? kResident8 : 4);
   Table<CAP> t;
   uint64_t chunks = 0;
   for (int i = 0; i < count; ++i) {
@@ -299,17 +453,20 @@ int launch(const nvfp4_adamw_tensor* ts, int count, const nvfp4_adamw_hyper* hs,
     t.e[i] = Entry{s.param, s.grad, s.first, s.second, static_cast<uint8_t*>(s.first_scale),
                    static_cast<uint8_t*>(s.second_scale), s.n, s.counter_base, s.hyper, wide};
     t.start[i] = (uint32_t)chunks;
-    chunks += (uint64_t)((s.n + kChunk - 1) / kChunk);
+    chunks += (uint64_t)((s.n + chunk - 1) / chunk);
     if (chunks > 0x7fffffffu) return NVFP4_E_LIMIT;
   }
   t.start[count] = (uint32_t)chunks;
   t.count = count;
   for (int i = 0; i < n_hypers; ++i) {
     const nvfp4_adamw_hyper& s = hs[i];
-    t.h[i] = Hyper{s.decay, s.beta1, s.rest1, s.beta2, s.rest2, s.step_size, s.inv_root_correction, s.eps, s.philox_offset};
+    auto two = [](float a) { return make_float2(a, a); };
+    t.h[i] = Hyper{two(s.decay), two(s.beta1), two(s.rest1), two(s.beta2), two(s.rest2), two(-s.step_size),
+                   two(s.inv_root_correction), two(s.eps), two(1.0f), s.philox_offset};
   }
-  const unsigned grid = (unsigned)(chunks < 148 * 4 ? chunks : 148 * 4);
-  adamw_kernel<T, EIGHT, CAP><<<grid, kThreads, 0, stream>>>(t, clip, keys);
+  const unsigned grid = (unsigned)(chunks < resident ? chunks : resident);
+  if constexpr (EIGHT) adamw8_kernel<T, CAP><<<grid, kThreads, 0, stream>>>(t, clip, keys);
+  else adamw_kernel<T, CAP><<<grid, kThreads, 0, stream>>>(t, clip);
   return cudaGetLastError() == cudaSuccess ? NVFP4_OK : NVFP4_E_LAUNCH;
 }
 
@@ -325,10 +482,10 @@ extern "C" int nvfp4_sumsq_parts(int count, const int64_t* counts) {
     uint64_t chunks = 0;
     for (int j = i; j < count && j < i + kNormCap; ++j) {
       if (counts[j] <= 0) return NVFP4_E_SHAPE;
-      chunks += (uint64_t)((counts[j] + kChunk - 1) / kChunk);
+      chunks += (uint64_t)((counts[j] + kNormChunk - 1) / kNormChunk);
     }
     if (chunks > 0x7fffffffu) return NVFP4_E_LIMIT;
-    parts += (int)(chunks < 148 * 4 ? chunks : 148 * 4);
+    parts += (int)(chunks < kNormGrid ? chunks : kNormGrid);
   }
   return parts;
 }
@@ -353,11 +510,11 @@ extern "C" int nvfp4_sumsq(const void* const* grads, const int64_t* counts, int 
       t.n[j] = counts[i + j];
       t.wide[j] = aligned(grads[i + j], is_f32 ? 32 : 16);
       t.start[j] = chunks;
-      chunks += (uint32_t)((counts[i + j] + kChunk - 1) / kChunk);
+      chunks += (uint32_t)((counts[i + j] + kNormChunk - 1) / kNormChunk);
     }
     t.start[m] = chunks;
     t.count = m;
-    const unsigned grid = chunks < 148 * 4 ? chunks : 148 * 4;
+    const unsigned grid = chunks < kNormGrid ? chunks : kNormGrid;
     if (is_f32) sumsq_kernel<float><<<grid, kThreads, 0, stream>>>(t, parts);
     else sumsq_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(t, parts);
     if (cudaGetLastError() != cudaSuccess) return NVFP4_E_LAUNCH;
@@ -406,10 +563,10 @@ extern "C" int nvfp4_adamw(const nvfp4_adamw_tensor* tensors, int count, const n
       constexpr int cap = decltype(small)::value;
       const nvfp4_adamw_tensor* ts = tensors + i;
       if (is_f32)
-        return eight ? launch<float, true, cap>(ts, m, hypers, n_hypers, clip, keys, stream)
-                     : launch<float, false, cap>(ts, m, hypers, n_hypers, clip, keys, stream);
-      return eight ? launch<__nv_bfloat16, true, cap>(ts, m, hypers, n_hypers, clip, keys, stream)
-                   : launch<__nv_bfloat16, false, cap>(ts, m, hypers, n_hypers, clip, keys, stream);
+        return eight ? launch_step<float, true, cap>(ts, m, hypers, n_hypers, clip, keys, stream)
+                     : launch_step<float, false, cap>(ts, m, hypers, n_hypers, clip, keys, stream);
+      return eight ? launch_step<__nv_bfloat16, true, cap>(ts, m, hypers, n_hypers, clip, keys, stream)
+                   : launch_step<__nv_bfloat16, false, cap>(ts, m, hypers, n_hypers, clip, keys, stream);
     };
     const int code = m <= kSmall ? go(std::integral_constant<int, kSmall>()) : go(std::integral_constant<int, kLarge>());
     if (code != NVFP4_OK) return code;

@@ -14,6 +14,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -27,7 +28,8 @@ namespace {
   F(nvfp4_amax_bf16) F(nvfp4_amax_both_bf16) F(nvfp4_quantize_fused_bf16) F(nvfp4_quantize_shard_bf16)                 \
   F(nvfp4_quantize_weight_bf16) F(nvfp4_quantize_dual_bf16) F(nvfp4_round_amax_f32) F(nvfp4_gemm) F(nvfp4_gemm_amax) \
   F(nvfp4_gemm_bf16_as_f32) F(nvfp4_adamw) F(nvfp4_sumsq) F(nvfp4_sumsq_parts) F(nvfp4_norm_of_sumsq)       \
-  F(nvfp4_logprob_fwd) F(nvfp4_logprob_bwd) F(nvfp4_preference_fwd) F(nvfp4_policy_fwd)
+  F(nvfp4_logprob_fwd) F(nvfp4_logprob_bwd) F(nvfp4_preference_fwd) F(nvfp4_policy_fwd)                         \
+  F(nvfp4_status_string)
 
 struct Library {
 #define F(name) decltype(&::name) name = nullptr;
@@ -428,11 +430,34 @@ py::object grad_norm(const py::list& params) {
   return py::cast(norm);
 }
 
-PyObject* item(PyObject* dict, const char* key) {
-  PyObject* v = PyDict_GetItemString(dict, key);
-  if (v == nullptr) raise(PyExc_KeyError, key);
+struct Name {                                               // an interned string: looked up by its address
+  PyObject* s;
+  explicit Name(const char* n) : s(PyUnicode_InternFromString(n)) {}
+};
+PyObject* item(PyObject* dict, const Name& key) {
+  PyObject* v = PyDict_GetItemWithError(dict, key.s);
+  if (v == nullptr) {
+    if (!PyErr_Occurred()) PyErr_SetObject(PyExc_KeyError, key.s);
+    throw py::error_already_set();
+  }
   return v;
 }
+// The entries of a dict whose keys come in the order they were put in: then no key is hashed (a tensor's hash is a Python call).
+struct InOrder {
+  PyObject* dict;
+  Py_ssize_t pos = 0;
+  PyObject* find(PyObject* key) {
+    PyObject *k = nullptr, *v = nullptr;
+    Py_ssize_t next = pos;
+    if (PyDict_Next(dict, &next, &k, &v) && k == key) {
+      pos = next;
+      return v;
+    }
+    v = PyDict_GetItemWithError(dict, key);
+    if (v == nullptr && PyErr_Occurred()) throw py::error_already_set();
+    return v;
+  }
+};
 double number(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw py::error_already_set();
@@ -456,6 +481,7 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
     int group, f32;
     int64_t step;
     PyObject* state;
+    c10::TensorImpl* param;
   };
   std::vector<Hyper> hypers;
   std::vector<Item> items;
@@ -464,13 +490,18 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
   c10::optional<c10::Device> dev;
   uint64_t base = 0;
   const bool eight = bits == 8;
+  static const Name kBetas("betas"), kLr("lr"), kEps("eps"), kDecay("weight_decay"), kParams("params"), kStep("step"),
+      kFirst("exp_avg"), kSecond("exp_avg_sq"), kRoot("exp_avg_root"), kFirstScale("exp_avg_scale"),
+      kRootScale("exp_avg_root_scale");
+  const at::NoGradGuard no_grad;
+  InOrder states{state.ptr()};
   for (py::handle gh : groups) {
     PyObject* group = gh.ptr();
     if (!PyDict_Check(group)) raise(PyExc_TypeError, "param_groups holds dicts");
-    const py::sequence betas = py::reinterpret_borrow<py::sequence>(item(group, "betas"));
-    hypers.push_back({number(item(group, "lr")), number(py::object(betas[0]).ptr()), number(py::object(betas[1]).ptr()),
-                      number(item(group, "eps")), number(item(group, "weight_decay"))});
-    for (py::handle ph : py::reinterpret_borrow<py::list>(item(group, "params"))) {
+    const py::sequence betas = py::reinterpret_borrow<py::sequence>(item(group, kBetas));
+    hypers.push_back({number(item(group, kLr)), number(py::object(betas[0]).ptr()), number(py::object(betas[1]).ptr()),
+                      number(item(group, kEps)), number(item(group, kDecay))});
+    for (py::handle ph : py::reinterpret_borrow<py::list>(item(group, kParams))) {
       const at::Tensor& p = tensor_of(ph.ptr());
       const int64_t n = p.numel(), blocks = (n + 255) / 256;
       const uint64_t at_ = base;
@@ -479,11 +510,8 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
       if (!g0.defined() || n == 0) continue;
       check_param(p, dev);
       at::Tensor g = grad_like(p, g0);
-      PyObject* st = PyDict_GetItemWithError(state.ptr(), ph.ptr());
-      if (st == nullptr) {
-        if (PyErr_Occurred()) throw py::error_already_set();
-        return py::bool_(false);
-      }
+      PyObject* st = states.find(ph.ptr());
+      if (st == nullptr) return py::bool_(false);
       if (!PyDict_Check(st)) raise(PyExc_TypeError, "optimizer state holds dicts");
       Item it{};
       it.t.param = p.data_ptr();
@@ -492,14 +520,15 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
       it.t.counter_base = at_;
       it.group = (int)hypers.size() - 1;
       it.f32 = p.scalar_type() == at::kFloat;
-      it.step = PyLong_AsLongLong(item(st, "step")) + 1;
+      it.step = PyLong_AsLongLong(item(st, kStep)) + 1;
       if (it.step == 0 && PyErr_Occurred()) throw py::error_already_set();
       it.state = st;
-      const at::Tensor& m = tensor_of(item(st, "exp_avg"));
-      const at::Tensor& v = tensor_of(item(st, eight ? "exp_avg_root" : "exp_avg_sq"));
+      it.param = p.unsafeGetTensorImpl();
+      const at::Tensor& m = tensor_of(item(st, kFirst));
+      const at::Tensor& v = tensor_of(item(st, eight ? kRoot : kSecond));
       if (eight) {
-        const at::Tensor& ms = tensor_of(item(st, "exp_avg_scale"));
-        const at::Tensor& vs = tensor_of(item(st, "exp_avg_root_scale"));
+        const at::Tensor& ms = tensor_of(item(st, kFirstScale));
+        const at::Tensor& vs = tensor_of(item(st, kRootScale));
         check_state(m, *dev, at::kFloat8_e4m3fn, blocks * 256, "exp_avg");
         check_state(v, *dev, at::kFloat8_e4m3fn, blocks * 256, "exp_avg_root");
         check_state(ms, *dev, at::kFloat8_e8m0fnu, blocks, "exp_avg_scale");
@@ -578,14 +607,9 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
   }
   for (const Item& it : items) {
     const py::int_ step(it.step);
-    if (PyDict_SetItemString(it.state, "step", step.ptr()) != 0) throw py::error_already_set();
+    if (PyDict_SetItem(it.state, kStep.s, step.ptr()) != 0) throw py::error_already_set();
+    it.param->bump_version();                                // it changed in place, as any optimizer changes it
   }
-  // the parameters changed in place, as any optimizer changes them
-  for (py::handle gh : groups)
-    for (py::handle ph : py::reinterpret_borrow<py::list>(item(gh.ptr(), "params"))) {
-      const at::Tensor& p = tensor_of(ph.ptr());
-      if (p.grad().defined()) p.unsafeGetTensorImpl()->bump_version();
-    }
   if (norm.defined()) return py::cast(norm);
   return py::bool_(true);
 }
@@ -622,69 +646,133 @@ struct Logits {
   }
 };
 
-py::tuple logprob_fwd(const at::Tensor& logits, const at::Tensor& labels, int64_t ignore) {
-  const Logits in(logits, labels, ignore);
-  const c10::cuda::CUDAGuard guard(in.dev);
-  at::Tensor logp = in.per_row(), lse = in.per_row();
-  check(lib.nvfp4_logprob_fwd(&in.rows, float_ptr(logp), float_ptr(lse), stream_of(in.dev)), "nvfp4_logprob_fwd");
-  return py::make_tuple(logp, lse);
-}
+// Nodes of the autograd graph.  In C++ because of the backward pass, which autograd runs on a thread of its own: a Python
+// node has to wait there for the interpreter lock (a loss of 48 logit rows and its gradient: 122 us, 68 us from here).
+using torch::autograd::AutogradContext;
+using torch::autograd::tensor_list;
 
-// weight: dloss / dlogp, one per row or one per sequence; scale: what it is to be multiplied with (one element); ready: the
-// gradient for a scale of 1, to be used again where the scale is 1
-at::Tensor logprob_bwd(const at::Tensor& logits, const at::Tensor& labels, int64_t ignore, const at::Tensor& lse,
-                       const at::Tensor& weight, const OptTensor& scale, const OptTensor& ready) {
-  const Logits in(logits, labels, ignore);
+void check_in_backward(int code, const char* what) {         // without the interpreter
+  if (code != 0) throw std::runtime_error(std::string(what) + " failed: " + lib.nvfp4_status_string(code));
+}
+void only_once(const tensor_list& grads) {
+  if (!c10::GradMode::is_enabled()) return;
+  for (const at::Tensor& g : grads)
+    if (g.defined() && g.requires_grad()) throw std::runtime_error("the losses on logits are differentiable once");
+}
+// Gradient of the logits.  saved: logits, labels, logsumexp, dloss / dlogp (one per row or per sequence); scale: what the
+// latter is to be multiplied with (one element); ready: the gradient for a scale of 1, used again where the scale is 1
+at::Tensor dlogits(const torch::autograd::variable_list& saved, int64_t ignore, const at::Tensor& weight, const at::Tensor& scale,
+                   const at::Tensor& ready) {
+  const Logits in(saved[0], saved[1], ignore);
   const c10::cuda::CUDAGuard guard(in.dev);
-  const at::Tensor w = in.vec(weight, weight.numel() == in.rows.batch ? in.rows.batch : in.count(), "weight");
-  at::Tensor sc;
-  if (scale.has_value()) sc = in.vec(*scale, 1, "scale");
-  at::Tensor out = ready.has_value() ? *ready : at::empty(logits.sizes(), on(in.dev, logits.scalar_type()));
-  check(lib.nvfp4_logprob_bwd(&in.rows, float_ptr(lse), float_ptr(w), in.count() / w.numel(), sc.defined() ? float_ptr(sc) : nullptr,
-                              ready.has_value(), out.data_ptr(), stream_of(in.dev)),
-        "nvfp4_logprob_bwd");
+  const at::Tensor w = weight.to(at::kFloat).contiguous(), sc = scale.defined() ? scale.to(at::kFloat) : scale;
+  at::Tensor out = ready.defined() ? ready : at::empty(saved[0].sizes(), on(in.dev, saved[0].scalar_type()));
+  check_in_backward(lib.nvfp4_logprob_bwd(&in.rows, float_ptr(saved[2]), float_ptr(w), in.count() / w.numel(),
+                                          sc.defined() ? float_ptr(sc) : nullptr, ready.defined(), out.data_ptr(), stream_of(in.dev)),
+                    "nvfp4_logprob_bwd");
   return out;
 }
 
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& labels, int64_t ignore) {
+    const Logits in(logits, labels, ignore);
+    const c10::cuda::CUDAGuard guard(in.dev);
+    at::Tensor logp = in.per_row(), lse = in.per_row();
+    check(lib.nvfp4_logprob_fwd(&in.rows, float_ptr(logp), float_ptr(lse), stream_of(in.dev)), "nvfp4_logprob_fwd");
+    ctx->save_for_backward({logits, labels, lse});
+    ctx->saved_data["ignore"] = ignore;
+    return logp;
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    only_once(grads);
+    return {dlogits(ctx->get_saved_variables(), ctx->saved_data["ignore"].toInt(), grads[0], {}, {}), {}, {}};
+  }
+};
+
 at::Tensor loss_workspace(c10::Device dev) { return at::empty({NVFP4_LOSS_WORKSPACE}, on(dev, at::kByte)); }
 
-// (loss, rewards, lse, weight)
-py::tuple preference_fwd(const at::Tensor& logits, const at::Tensor& labels, int64_t ignore, const at::Tensor& ref, double beta,
-                         double smoothing) {
-  const Logits in(logits, labels, ignore);
-  const c10::cuda::CUDAGuard guard(in.dev);
-  if (logits.dim() != 3 || in.rows.batch % 2 != 0)
-    raise(PyExc_ValueError, "logits must be [2 pairs, seq, vocab], the chosen sequences first");
-  const at::Tensor r = in.vec(ref, in.rows.batch, "ref_logps");
-  at::Tensor logp = at::empty({in.count()}, on(in.dev, at::kDouble)), lse = in.per_row(), loss = at::empty({}, on(in.dev, at::kFloat)),
-             rewards = at::empty({in.rows.batch}, on(in.dev, at::kFloat)), weight = at::empty_like(rewards);
-  const at::Tensor ws = loss_workspace(in.dev);
-  check(lib.nvfp4_preference_fwd(&in.rows, float_ptr(r), beta, smoothing, static_cast<double*>(logp.data_ptr()), float_ptr(lse), float_ptr(loss),
-                                 float_ptr(rewards), float_ptr(weight), ws.data_ptr(), ws.numel(), stream_of(in.dev)),
-        "nvfp4_preference_fwd");
-  return py::make_tuple(loss, rewards, lse, weight);
-}
+// -> loss, rewards
+struct Preference : torch::autograd::Function<Preference> {
+  static tensor_list forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& labels, const at::Tensor& ref,
+                             double beta, double smoothing, int64_t ignore) {
+    const Logits in(logits, labels, ignore);
+    if (logits.dim() != 3 || in.rows.batch % 2 != 0)
+      raise(PyExc_ValueError, "logits must be [2 pairs, seq, vocab], the chosen sequences first");
+    const at::Tensor r = in.vec(ref, in.rows.batch, "ref_logps");
+    const c10::cuda::CUDAGuard guard(in.dev);
+    at::Tensor logp = at::empty({in.count()}, on(in.dev, at::kDouble)), lse = in.per_row(), loss = at::empty({}, on(in.dev, at::kFloat)),
+               rewards = at::empty({in.rows.batch}, on(in.dev, at::kFloat)), weight = at::empty_like(rewards);
+    const at::Tensor ws = loss_workspace(in.dev);
+    check(lib.nvfp4_preference_fwd(&in.rows, float_ptr(r), beta, smoothing, static_cast<double*>(logp.data_ptr()), float_ptr(lse),
+                                   float_ptr(loss), float_ptr(rewards), float_ptr(weight), ws.data_ptr(), ws.numel(),
+                                   stream_of(in.dev)),
+          "nvfp4_preference_fwd");
+    ctx->save_for_backward({logits, labels, lse, weight});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->mark_non_differentiable({rewards});
+    return {loss, rewards};
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    only_once(grads);
+    const auto saved = ctx->get_saved_variables();
+    return {dlogits(saved, ctx->saved_data["ignore"].toInt(), saved[3], grads[0], {}), {}, {}, {}, {}, {}};
+  }
+};
 
-// (loss, stats, logp, lse, weight, gradient of the logits or None)
-py::tuple policy_fwd(const at::Tensor& logits, const at::Tensor& labels, int64_t ignore, const at::Tensor& old_logps,
-                     const at::Tensor& advantages, const OptTensor& ref, double low, double high, double kl, bool want_grad) {
-  const Logits in(logits, labels, ignore);
-  const c10::cuda::CUDAGuard guard(in.dev);
-  const int64_t n = in.count();
-  const bool per_sequence = advantages.dim() == 1 && logits.dim() == 3;
-  const at::Tensor old = in.vec(old_logps, n, "old_logps"),
-                   adv = in.vec(advantages, per_sequence ? in.rows.batch : n, "advantages");
-  at::Tensor rf, grad;
-  if (ref.has_value()) rf = in.vec(*ref, n, "ref_logps");
-  at::Tensor logp = in.per_row(), lse = in.per_row(), weight = in.per_row(), loss = at::empty({}, on(in.dev, at::kFloat)),
-             stats = at::empty({2}, on(in.dev, at::kFloat));
-  if (want_grad) grad = at::empty(logits.sizes(), on(in.dev, logits.scalar_type()));
-  const at::Tensor ws = loss_workspace(in.dev);
-  check(lib.nvfp4_policy_fwd(&in.rows, float_ptr(old), float_ptr(adv), n / adv.numel(), rf.defined() ? float_ptr(rf) : nullptr, low,
-                             high, kl, float_ptr(logp), float_ptr(lse), float_ptr(weight), float_ptr(loss), float_ptr(stats),
-                             want_grad ? grad.data_ptr() : nullptr, ws.data_ptr(), ws.numel(), stream_of(in.dev)),
-        "nvfp4_policy_fwd");
-  return py::make_tuple(loss, stats, logp, lse, weight, want_grad ? py::cast(grad) : py::none());
+// -> loss, stats, log-probabilities.  The forward kernel writes the gradient for dloss = 1 while it has the rows at hand;
+// the backward writes it again only where the loss arrives with another factor.
+struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
+  static tensor_list forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& labels, const at::Tensor& old_logps,
+                             const at::Tensor& advantages, const OptTensor& ref, double low, double high, double kl,
+                             int64_t ignore, bool want_grad) {
+    const Logits in(logits, labels, ignore);
+    const int64_t n = in.count();
+    const bool per_sequence = advantages.dim() == 1 && logits.dim() == 3;
+    const at::Tensor old = in.vec(old_logps, n, "old_logps"),
+                     adv = in.vec(advantages, per_sequence ? in.rows.batch : n, "advantages");
+    at::Tensor rf, grad;
+    if (ref.has_value()) rf = in.vec(*ref, n, "ref_logps");
+    const c10::cuda::CUDAGuard guard(in.dev);
+    at::Tensor logp = in.per_row(), lse = in.per_row(), weight = in.per_row(), loss = at::empty({}, on(in.dev, at::kFloat)),
+               stats = at::empty({2}, on(in.dev, at::kFloat));
+    if (want_grad) grad = at::empty(logits.sizes(), on(in.dev, logits.scalar_type()));
+    const at::Tensor ws = loss_workspace(in.dev);
+    check(lib.nvfp4_policy_fwd(&in.rows, float_ptr(old), float_ptr(adv), n / adv.numel(), rf.defined() ? float_ptr(rf) : nullptr,
+                               low, high, kl, float_ptr(logp), float_ptr(lse), float_ptr(weight), float_ptr(loss), float_ptr(stats),
+                               want_grad ? grad.data_ptr() : nullptr, ws.data_ptr(), ws.numel(), stream_of(in.dev)),
+          "nvfp4_policy_fwd");
+    ctx->save_for_backward({logits, labels, lse, weight});
+    ctx->saved_data["ignore"] = ignore;
+    if (want_grad) ctx->saved_data["grad"] = grad;
+    ctx->mark_non_differentiable({stats, logp});
+    return {loss, stats, logp};
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    only_once(grads);
+    const auto saved = ctx->get_saved_variables();
+    at::Tensor ready;
+    if (auto it = ctx->saved_data.find("grad"); it != ctx->saved_data.end()) {      // (a second backward writes its own)
+      ready = it->second.toTensor();
+      ctx->saved_data.erase(it);
+    }
+    return {dlogits(saved, ctx->saved_data["ignore"].toInt(), saved[3], grads[0], ready), {}, {}, {}, {}, {}, {}, {}, {}, {}};
+  }
+};
+
+at::Tensor token_logprobs(const at::Tensor& logits, const at::Tensor& labels, int64_t ignore) {
+  return TokenLogprobs::apply(logits, labels, ignore);
+}
+py::tuple preference_loss(const at::Tensor& logits, const at::Tensor& labels, const at::Tensor& ref, double beta, double smoothing,
+                          int64_t ignore) {
+  const tensor_list out = Preference::apply(logits, labels, ref, beta, smoothing, ignore);
+  const int64_t pairs = out[1].numel() / 2;
+  return py::make_tuple(out[0], out[1].narrow(0, 0, pairs), out[1].narrow(0, pairs, pairs));
+}
+py::tuple policy_loss(const at::Tensor& logits, const at::Tensor& labels, const at::Tensor& old_logps, const at::Tensor& advantages,
+                      const OptTensor& ref, double low, double high, double kl, int64_t ignore) {
+  const bool want_grad = c10::GradMode::is_enabled() && logits.requires_grad();
+  const tensor_list out = PolicyLoss::apply(logits, labels, old_logps, advantages, ref, low, high, kl, ignore, want_grad);
+  return py::make_tuple(out[0], out[2], out[1].select(0, 0), out[1].select(0, 1));
 }
 
 }  // namespace
@@ -703,8 +791,7 @@ PYBIND11_MODULE(_host, m) {
   m.def("mm_bf16_as_f32", &mm_bf16_as_f32);
   m.def("grad_norm", &grad_norm);
   m.def("adamw_step", &adamw_step);
-  m.def("logprob_fwd", &logprob_fwd);
-  m.def("logprob_bwd", &logprob_bwd);
-  m.def("preference_fwd", &preference_fwd);
-  m.def("policy_fwd", &policy_fwd);
+  m.def("token_logprobs", &token_logprobs);
+  m.def("preference_loss", &preference_loss);
+  m.def("policy_loss", &policy_loss);
 }

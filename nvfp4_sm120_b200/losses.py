@@ -10,74 +10,14 @@ the logits' dtype.  Gradients are those of the logits: every other argument is a
 The reference trains with cross-entropy alone (nvfp4_train.py:159-185)."""
 from __future__ import annotations
 
-import torch
-from torch.autograd.function import once_differentiable
-
 from . import _lib
 
 IGNORE_INDEX = -100
 
 
-class TokenLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, ignore_index):
-        logp, lse = _lib.host().logprob_fwd(logits, labels, ignore_index)
-        ctx.save_for_backward(logits, labels, lse)
-        ctx.ignore_index = ignore_index
-        return logp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dlogp):
-        logits, labels, lse = ctx.saved_tensors
-        return _lib.host().logprob_bwd(logits, labels, ctx.ignore_index, lse, dlogp.reshape(-1), None, None), None, None
-
-
-class PreferenceFn(torch.autograd.Function):
-    """-> (loss, rewards [2 pairs])"""
-
-    @staticmethod
-    def forward(ctx, logits, labels, ref_logps, beta, label_smoothing, ignore_index):
-        loss, rewards, lse, weight = _lib.host().preference_fwd(logits, labels, ignore_index, ref_logps, beta, label_smoothing)
-        ctx.save_for_backward(logits, labels, lse, weight)
-        ctx.ignore_index = ignore_index
-        ctx.mark_non_differentiable(rewards)
-        return loss, rewards
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dloss, _):
-        logits, labels, lse, weight = ctx.saved_tensors
-        d = _lib.host().logprob_bwd(logits, labels, ctx.ignore_index, lse, weight, dloss, None)
-        return d, None, None, None, None, None
-
-
-class PolicyFn(torch.autograd.Function):
-    """-> (loss, stats [2], log-probabilities).  The forward kernel writes the gradient for dloss = 1 while it has the
-    rows at hand; the backward writes it again only where the loss arrives with another factor."""
-
-    @staticmethod
-    def forward(ctx, logits, labels, old_logps, advantages, ref_logps, clip, clip_high, kl_coef, ignore_index, grad_on):
-        loss, stats, logp, lse, weight, grad = _lib.host().policy_fwd(logits, labels, ignore_index, old_logps, advantages,
-                                                                      ref_logps, clip, clip_high, kl_coef,
-                                                                      grad_on and ctx.needs_input_grad[0])
-        ctx.save_for_backward(logits, labels, lse, weight)
-        ctx.ignore_index, ctx.grad = ignore_index, grad
-        ctx.mark_non_differentiable(stats, logp)
-        return loss, stats, logp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dloss, _stats, _logp):
-        logits, labels, lse, weight = ctx.saved_tensors
-        ready, ctx.grad = ctx.grad, None            # (a second backward writes its own)
-        d = _lib.host().logprob_bwd(logits, labels, ctx.ignore_index, lse, weight, dloss, ready)
-        return d, None, None, None, None, None, None, None, None, None
-
-
 def token_logprobs(logits, labels, ignore_index=IGNORE_INDEX):
     """log softmax(logits)[label] in fp32, of the labels' shape; 0 where the label is ignored."""
-    return TokenLogprobsFn.apply(logits, labels, int(ignore_index))
+    return _lib.host().token_logprobs(logits, labels, int(ignore_index))
 
 
 def preference_loss(logits, labels, ref_logps, beta=0.1, label_smoothing=0.0, ignore_index=IGNORE_INDEX):
@@ -89,9 +29,7 @@ def preference_loss(logits, labels, ref_logps, beta=0.1, label_smoothing=0.0, ig
     -(1 - label_smoothing) logsigmoid(h) - label_smoothing logsigmoid(-h)."""
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"label_smoothing must lie in [0, 1], got {label_smoothing}")
-    loss, rewards = PreferenceFn.apply(logits, labels, ref_logps, float(beta), float(label_smoothing), int(ignore_index))
-    chosen, rejected = rewards.chunk(2)
-    return loss, chosen, rejected
+    return _lib.host().preference_loss(logits, labels, ref_logps, float(beta), float(label_smoothing), int(ignore_index))
 
 
 def policy_loss(logits, labels, old_logps, advantages, ref_logps=None, clip=0.2, clip_high=None, kl_coef=0.0,
@@ -112,6 +50,6 @@ def policy_loss(logits, labels, old_logps, advantages, ref_logps=None, clip=0.2,
         raise ValueError(f"clip must lie in [0, 1] and clip_high must not be negative, got {clip} and {clip_high}")
     if kl_coef and ref_logps is None:
         raise ValueError("kl_coef needs ref_logps")
-    loss, stats, logps = PolicyFn.apply(logits, labels, old_logps, advantages, ref_logps, float(clip), float(clip_high),
-                                        float(kl_coef), int(ignore_index), torch.is_grad_enabled())
-    return loss, {"logps": logps, "kl": stats[0], "clip_fraction": stats[1]}
+    loss, logps, kl, fraction = _lib.host().policy_loss(logits, labels, old_logps, advantages, ref_logps, float(clip),
+                                                        float(clip_high), float(kl_coef), int(ignore_index))
+    return loss, {"logps": logps, "kl": kl, "clip_fraction": fraction}

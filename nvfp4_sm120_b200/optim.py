@@ -124,7 +124,6 @@ class AdamW(torch.optim.Optimizer):
                         mine[n].copy_(st[n])
 
     # ---- step ----
-    @torch.no_grad()
     def step(self, closure=None, *, grad_norm=None):
         """One step of every parameter that has a gradient.  grad_norm: one fp32 element on the parameters' device to
         clip by, in place of the norm found here."""

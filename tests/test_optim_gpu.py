@@ -233,8 +233,14 @@ def test_eight_bit_moments(optim, n, dtype):
         first.grad = torch.ones_like(first)
         before = p.detach().clone()
         opt.step()
-        po, mo, vo = _operations(before, p.grad, m, v, t, 3e-3, 0.9, 0.95, 1e-8, 0.1)
-        assert torch.equal(p.detach(), po)
+        args = (before, p.grad, m, v, t, 3e-3, 0.9, 0.95, 1e-8, 0.1)
+        (po, _, _), (_, mo, vo) = _formula(*args), _operations(*args)
+        # approximate root and reciprocal (2^-23 and 2^-22.5) and a dozen roundings on the update, two on the weight, the
+        # rounding to its dtype; the update is at most lr / (1 - b1^t) times (root / sqrt(1 - b2^t))^-1 of the terms of m
+        update = 3e-3 / (1 - 0.9 ** t) * (0.9 * m.double().abs() + 0.1 * p.grad.double().abs()) / (
+            vo.double().sqrt() / math.sqrt(1 - 0.95 ** t) + 1e-8)
+        assert ((p.detach().double() - po).abs() <= torch.finfo(dtype).eps / 2 * 1.001 * po.abs()
+                + 2.0 ** -24 * 3 * before.double().abs() + 2.0 ** -20 * update).all()
         st = opt.state[p]
         bits = _dither(blocks * 32, t, seed, base=2 * 32)
         pad = lambda x: torch.cat([x, x.new_zeros(blocks * BLOCK - n)]).view(blocks, BLOCK)

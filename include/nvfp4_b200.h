@@ -425,7 +425,7 @@ int nvfp4_norm_of_sumsq(const double* parts, int n_parts, float* norm, void* str
 /*
  * Losses on logits [batch, seq, vocab] (fp32, or bf16 when is_f32 == 0; strides in elements, the logits of a row contiguous;
  * rows are numbered batch * seq + position).  A row whose label equals ignore_index has no part in anything and is not read;
- * any other label outside [0, vocab) gives NaN.  All row and sequence vectors are fp32.
+ * any other label outside [0, vocab) gives NaN.  At most 2^31 - 1 rows of at most 2^31 - 1 logits.  All row and sequence vectors are fp32.
  */
 typedef struct {
   const void* logits;
@@ -437,17 +437,19 @@ typedef struct {
 } nvfp4_logit_rows;           /* HOST struct, read before the call returns */
 /* Scratch of the calls that return a loss: device memory, 16-byte aligned, any content; calls that share it must not overlap. */
 #define NVFP4_LOSS_PARTS 1184
-#define NVFP4_LOSS_WORKSPACE (16 + 3 * 8 * NVFP4_LOSS_PARTS)
+#define NVFP4_LOSS_WORKSPACE (1024 + 4 * 8 * NVFP4_LOSS_PARTS)
 
 /*
  * logp[row] = x[label] - lse, lse[row] = log sum exp of the row (both 0 for an ignored row).
- * Backward: dlogits (contiguous [batch, seq, vocab], the logits' type) = w (onehot(label) - exp(x - lse)), w =
+ * Backward: dlogits ([batch, seq, vocab] of the logits' type with strides of its own, rows that do not overlap; fastest where each
+ * row lies as its logits do modulo 16 bytes) = w (onehot(label) - exp(x - lse)), w =
  * weight[row / rows_per_weight] (* *scale when given).  unless_one != 0: dlogits already holds the result for a scale of 1, and the
  * call leaves it alone when *scale is 1.  The reference uses torch's cross_entropy (nvfp4_train.py:159-185).
  */
 int nvfp4_logprob_fwd(const nvfp4_logit_rows* rows, float* logp, float* lse, void* stream);
 int nvfp4_logprob_bwd(const nvfp4_logit_rows* rows, const float* lse, const float* weight, int64_t rows_per_weight,
-                      const float* scale, int unless_one, void* dlogits, void* stream);
+                      const float* scale, int unless_one, void* dlogits, int64_t dstride_b, int64_t dstride_t,
+                      void* stream);
 
 /*
  * Preference loss of batch / 2 pairs, sequence i chosen over sequence batch / 2 + i: with L_i the sum of the sequence's logp (fp64 here,
@@ -465,12 +467,13 @@ int nvfp4_preference_fwd(const nvfp4_logit_rows* rows, const float* ref, double 
  * loss = 1/n sum over the n rows with a label (n = 1 if there are none) of
  *   -min(rho A, clamp(rho, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1)     (no KL term when ref_logp is NULL)
  * stats2 = {mean of exp(d) - d - 1, share of rows whose clamp cut the gradient}; weight[row] = dloss / dlogp.
- * dlogits: NULL, or the gradient of the loss for nvfp4_logprob_bwd's layout, written while the row is in L2.
+ * terms: scratch [2, batch * seq].  dlogits: NULL, or the gradient of the loss in nvfp4_logprob_bwd's layout, written while the row is on chip.
  * No counterpart in the reference.
  */
 int nvfp4_policy_fwd(const nvfp4_logit_rows* rows, const float* old_logp, const float* advantage, int64_t rows_per_advantage,
                      const float* ref_logp, double clip_low, double clip_high, double kl, float* logp, float* lse, float* weight,
-                     float* loss, float* stats2, void* dlogits, void* workspace, size_t workspace_bytes, void* stream);
+                     float* terms, float* loss, float* stats2, void* dlogits, int64_t dstride_b, int64_t dstride_t,
+                     void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Test hooks of the bounded waits, process-wide, for the launches that follow.  Every spin inside

@@ -78,12 +78,12 @@ _SIGS = {
     "nvfp4_norm_of_sumsq": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_void_p, _c.c_void_p]),
     "nvfp4_logprob_fwd": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p]),
     "nvfp4_logprob_bwd": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int, _c.c_void_p,
-                                     _c.c_void_p]),
+                                     _c.c_int64, _c.c_int64, _c.c_void_p]),
     "nvfp4_preference_fwd": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_double, _c.c_double, _c.c_void_p, _c.c_void_p,
                                         _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
     "nvfp4_policy_fwd": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_double, _c.c_double,
                                     _c.c_double, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
-                                    _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+                                    _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
     "nvfp4_test_hooks": (_c.c_int, [_c.c_uint64, _c.c_int, _c.c_int]),
     "nvfp4_gemm_amax": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
                                    _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64,

@@ -646,6 +646,23 @@ struct Logits {
   }
 };
 
+// A tensor for the gradient of logits whose rows lie as the logits' own do, modulo 16 bytes: then both are read and written in
+// whole vectors.  (A view of shifted logits has rows at other places than a contiguous tensor of its shape.)
+at::Tensor gradient_like(const at::Tensor& x, const Logits& in) {
+  const nvfp4_logit_rows& r = in.rows;
+  const bool time_inside = r.stride_t <= r.stride_b || r.batch == 1;
+  const int64_t inner = time_inside ? r.stride_t : r.stride_b, outer = time_inside ? r.stride_b : r.stride_t;
+  const int64_t n_inner = time_inside ? r.seq : r.batch, n_outer = time_inside ? r.batch : r.seq;
+  const bool apart = (n_inner == 1 || inner >= r.vocab) && (n_outer == 1 || outer >= (n_inner - 1) * inner + r.vocab);
+  const int64_t span = (n_outer - 1) * outer + (n_inner - 1) * inner + r.vocab;
+  const int64_t shift = (int64_t)(reinterpret_cast<uintptr_t>(r.logits) % 16) / (r.is_f32 ? 4 : 2);
+  const auto opt = on(in.dev, x.scalar_type());
+  if (!apart || !in.x.is_same(x) || span > 2 * x.numel()) return at::empty(x.sizes(), opt);
+  if (shift == 0 && x.is_contiguous()) return at::empty(x.sizes(), opt);
+  return at::empty({span + shift}, opt).as_strided(x.sizes(), x.strides(), shift);
+}
+int64_t batch_stride(const at::Tensor& t) { return t.dim() == 3 ? t.stride(0) : 0; }
+
 // Nodes of the autograd graph.  In C++ because of the backward pass, which autograd runs on a thread of its own: a Python
 // node has to wait there for the interpreter lock (a loss of 48 logit rows and its gradient: 122 us, 68 us from here).
 using torch::autograd::AutogradContext;
@@ -659,16 +676,21 @@ void only_once(const tensor_list& grads) {
   for (const at::Tensor& g : grads)
     if (g.defined() && g.requires_grad()) throw std::runtime_error("the losses on logits are differentiable once");
 }
-// Gradient of the logits.  saved: logits, labels, logsumexp, dloss / dlogp (one per row or per sequence); scale: what the
-// latter is to be multiplied with (one element); ready: the gradient for a scale of 1, used again where the scale is 1
+// Gradient of the logits.  saved: logits, labels and, in one tensor, the rows' logsumexp and dloss / dlogp (one per row or per
+// sequence), or the former alone and `weight` for the latter; scale: what dloss / dlogp is to be multiplied with (one
+// element); ready: the gradient for a scale of 1, used again where the scale is 1
 at::Tensor dlogits(const torch::autograd::variable_list& saved, int64_t ignore, const at::Tensor& weight, const at::Tensor& scale,
                    const at::Tensor& ready) {
   const Logits in(saved[0], saved[1], ignore);
   const c10::cuda::CUDAGuard guard(in.dev);
-  const at::Tensor w = weight.to(at::kFloat).contiguous(), sc = scale.defined() ? scale.to(at::kFloat) : scale;
-  at::Tensor out = ready.defined() ? ready : at::empty(saved[0].sizes(), on(in.dev, saved[0].scalar_type()));
-  check_in_backward(lib.nvfp4_logprob_bwd(&in.rows, float_ptr(saved[2]), float_ptr(w), in.count() / w.numel(),
-                                          sc.defined() ? float_ptr(sc) : nullptr, ready.defined(), out.data_ptr(), stream_of(in.dev)),
+  const int64_t n = in.count();
+  const at::Tensor w = weight.defined() ? weight.to(at::kFloat).contiguous() : saved[2],
+                   sc = scale.defined() ? scale.to(at::kFloat) : scale;
+  const float* wp = float_ptr(w) + (weight.defined() ? 0 : n);
+  const int64_t per = n / (weight.defined() ? n : saved[2].numel() - n);
+  at::Tensor out = ready.defined() ? ready : gradient_like(saved[0], in);
+  check_in_backward(lib.nvfp4_logprob_bwd(&in.rows, float_ptr(saved[2]), wp, per, sc.defined() ? float_ptr(sc) : nullptr,
+                                          ready.defined(), out.data_ptr(), batch_stride(out), out.stride(-2), stream_of(in.dev)),
                     "nvfp4_logprob_bwd");
   return out;
 }
@@ -689,7 +711,8 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   }
 };
 
-at::Tensor loss_workspace(c10::Device dev) { return at::empty({NVFP4_LOSS_WORKSPACE}, on(dev, at::kByte)); }
+// scratch of a loss: the workspace and `more` bytes behind it
+at::Tensor loss_scratch(c10::Device dev, int64_t more) { return at::empty({NVFP4_LOSS_WORKSPACE + more}, on(dev, at::kByte)); }
 
 // -> loss, rewards
 struct Preference : torch::autograd::Function<Preference> {
@@ -700,22 +723,24 @@ struct Preference : torch::autograd::Function<Preference> {
       raise(PyExc_ValueError, "logits must be [2 pairs, seq, vocab], the chosen sequences first");
     const at::Tensor r = in.vec(ref, in.rows.batch, "ref_logps");
     const c10::cuda::CUDAGuard guard(in.dev);
-    at::Tensor logp = at::empty({in.count()}, on(in.dev, at::kDouble)), lse = in.per_row(), loss = at::empty({}, on(in.dev, at::kFloat)),
-               rewards = at::empty({in.rows.batch}, on(in.dev, at::kFloat)), weight = at::empty_like(rewards);
-    const at::Tensor ws = loss_workspace(in.dev);
-    check(lib.nvfp4_preference_fwd(&in.rows, float_ptr(r), beta, smoothing, static_cast<double*>(logp.data_ptr()), float_ptr(lse),
-                                   float_ptr(loss), float_ptr(rewards), float_ptr(weight), ws.data_ptr(), ws.numel(),
+    const int64_t n = in.count();
+    at::Tensor loss = at::empty({}, on(in.dev, at::kFloat)), rewards = at::empty({in.rows.batch}, on(in.dev, at::kFloat)),
+               kept = at::empty({n + in.rows.batch}, on(in.dev, at::kFloat));
+    const at::Tensor scratch = loss_scratch(in.dev, 8 * n);
+    uint8_t* ws = scratch.data_ptr<uint8_t>();
+    check(lib.nvfp4_preference_fwd(&in.rows, float_ptr(r), beta, smoothing, reinterpret_cast<double*>(ws + NVFP4_LOSS_WORKSPACE),
+                                   float_ptr(kept), float_ptr(loss), float_ptr(rewards), float_ptr(kept) + n, ws, NVFP4_LOSS_WORKSPACE,
                                    stream_of(in.dev)),
           "nvfp4_preference_fwd");
-    ctx->save_for_backward({logits, labels, lse, weight});
+    ctx->save_for_backward({logits, labels, kept});
     ctx->saved_data["ignore"] = ignore;
     ctx->mark_non_differentiable({rewards});
+    ctx->set_materialize_grads(false);
     return {loss, rewards};
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
     only_once(grads);
-    const auto saved = ctx->get_saved_variables();
-    return {dlogits(saved, ctx->saved_data["ignore"].toInt(), saved[3], grads[0], {}), {}, {}, {}, {}, {}};
+    return {dlogits(ctx->get_saved_variables(), ctx->saved_data["ignore"].toInt(), {}, grads[0], {}), {}, {}, {}, {}, {}};
   }
 };
 
@@ -733,29 +758,32 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     at::Tensor rf, grad;
     if (ref.has_value()) rf = in.vec(*ref, n, "ref_logps");
     const c10::cuda::CUDAGuard guard(in.dev);
-    at::Tensor logp = in.per_row(), lse = in.per_row(), weight = in.per_row(), loss = at::empty({}, on(in.dev, at::kFloat)),
+    at::Tensor logp = in.per_row(), kept = at::empty({2 * n}, on(in.dev, at::kFloat)), loss = at::empty({}, on(in.dev, at::kFloat)),
                stats = at::empty({2}, on(in.dev, at::kFloat));
-    if (want_grad) grad = at::empty(logits.sizes(), on(in.dev, logits.scalar_type()));
-    const at::Tensor ws = loss_workspace(in.dev);
+    if (want_grad) grad = gradient_like(logits, in);
+    const at::Tensor scratch = loss_scratch(in.dev, 8 * n);
+    uint8_t* ws = scratch.data_ptr<uint8_t>();
     check(lib.nvfp4_policy_fwd(&in.rows, float_ptr(old), float_ptr(adv), n / adv.numel(), rf.defined() ? float_ptr(rf) : nullptr,
-                               low, high, kl, float_ptr(logp), float_ptr(lse), float_ptr(weight), float_ptr(loss), float_ptr(stats),
-                               want_grad ? grad.data_ptr() : nullptr, ws.data_ptr(), ws.numel(), stream_of(in.dev)),
+                               low, high, kl, float_ptr(logp), float_ptr(kept), float_ptr(kept) + n,
+                               reinterpret_cast<float*>(ws + NVFP4_LOSS_WORKSPACE), float_ptr(loss), float_ptr(stats),
+                               want_grad ? grad.data_ptr() : nullptr, want_grad ? batch_stride(grad) : 0,
+                               want_grad ? grad.stride(-2) : 0, ws, NVFP4_LOSS_WORKSPACE, stream_of(in.dev)),
           "nvfp4_policy_fwd");
-    ctx->save_for_backward({logits, labels, lse, weight});
+    ctx->save_for_backward({logits, labels, kept});
     ctx->saved_data["ignore"] = ignore;
     if (want_grad) ctx->saved_data["grad"] = grad;
     ctx->mark_non_differentiable({stats, logp});
+    ctx->set_materialize_grads(false);
     return {loss, stats, logp};
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
     only_once(grads);
-    const auto saved = ctx->get_saved_variables();
     at::Tensor ready;
     if (auto it = ctx->saved_data.find("grad"); it != ctx->saved_data.end()) {      // (a second backward writes its own)
       ready = it->second.toTensor();
       ctx->saved_data.erase(it);
     }
-    return {dlogits(saved, ctx->saved_data["ignore"].toInt(), saved[3], grads[0], ready), {}, {}, {}, {}, {}, {}, {}, {}, {}};
+    return {dlogits(ctx->get_saved_variables(), ctx->saved_data["ignore"].toInt(), {}, grads[0], ready), {}, {}, {}, {}, {}, {}, {}, {}, {}};
   }
 };
 

@@ -25,7 +25,7 @@
 namespace nvfp4 {
 namespace logprob {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;                     // of the CTAs whose rows belong to warps, and of those that add up
 constexpr int kWarpRow = 2048;
 // log2 e in two parts: alone, the first is off by 1.3e-8 of itself, which moves every term of a row the same way, and the sum
 // of a sequence's thousand log-probabilities shows it.  (The mean error of a row's logsumexp, measured over 2048 rows of 13
@@ -51,6 +51,24 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 __device__ __forceinline__ float exp_of(float d) { return ex2(fmaf(d, kLog2e, d * kLog2eRest)); }
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+// the same of two, in packed instructions
+__device__ __forceinline__ float2 exp_of(float2 d) {
+  const float2 t = __ffma2_rn(d, both(kLog2e), __fmul2_rn(d, both(kLog2eRest)));
+  return make_float2(ex2(t.x), ex2(t.y));
+}
+// the same within 1.3e-8 d of itself: enough for a gradient
+__device__ __forceinline__ float exp_near(float d) { return ex2(d * kLog2e); }
+__device__ __forceinline__ float2 exp_near(float2 d) {
+  const float2 t = __fmul2_rn(d, both(kLog2e));
+  return make_float2(ex2(t.x), ex2(t.y));
+}
+// max(m, a, b) as one three-input instruction (a NaN does not count; it shows in the sum)
+__device__ __forceinline__ float max3(float m, float a, float b) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
+  return r;
+}
 // M + log s.  The sum's exponent is taken off in front of the logarithm, whose own rounding is then far below that of an fp32
 // result.  (Beside a coarse maximum, logf(s) would leave every other result halfway between two fp32 numbers.)
 __device__ __forceinline__ double lse_of(Stat st) {
@@ -59,29 +77,31 @@ __device__ __forceinline__ double lse_of(Stat st) {
   return (double)st.m + (k * 0.69314718055994531 + (double)logf(f));
 }
 
+// A 16-byte vector of logits as pairs of fp32, and back.
 template <class T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int n = 4;
-  static __device__ __forceinline__ void open(const uint4& q, float (&v)[4]) {
-    v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y); v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
+  static __device__ __forceinline__ void open(const uint4& q, float2* v) {
+    v[0] = make_float2(__uint_as_float(q.x), __uint_as_float(q.y));
+    v[1] = make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
   }
-  static __device__ __forceinline__ uint4 close(const float (&v)[4]) {
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  static __device__ __forceinline__ uint4 close(const float2* v) {
+    return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
   }
 };
-__device__ __forceinline__ uint32_t pack(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+__device__ __forceinline__ uint32_t pack(float2 a) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a.x, a.y);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int n = 8;
-  static __device__ __forceinline__ void open(const uint4& q, float (&v)[8]) {
-    v[0] = bf16_lo(q.x); v[1] = bf16_hi(q.x); v[2] = bf16_lo(q.y); v[3] = bf16_hi(q.y);
-    v[4] = bf16_lo(q.z); v[5] = bf16_hi(q.z); v[6] = bf16_lo(q.w); v[7] = bf16_hi(q.w);
+  static __device__ __forceinline__ void open(const uint4& q, float2* v) {
+    v[0] = make_float2(bf16_lo(q.x), bf16_hi(q.x));
+    v[1] = make_float2(bf16_lo(q.y), bf16_hi(q.y));
+    v[2] = make_float2(bf16_lo(q.z), bf16_hi(q.z));
+    v[3] = make_float2(bf16_lo(q.w), bf16_hi(q.w));
   }
-  static __device__ __forceinline__ uint4 close(const float (&v)[8]) {
-    return make_uint4(pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7]));
-  }
+  static __device__ __forceinline__ uint4 close(const float2* v) { return make_uint4(pack(v[0]), pack(v[1]), pack(v[2]), pack(v[3])); }
 };
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -96,42 +116,66 @@ template <class T> __device__ __forceinline__ uint32_t lead(const T* p, uint32_t
 }
 
 // ---- reading a row -----------------------------------------------------------------------------------------------------
-template <int N> __device__ __forceinline__ void take(Stat& st, const float (&v)[N]) {
-  float m = st.m;
-#pragma unroll
-  for (int j = 0; j < N; ++j) m = fmaxf(m, v[j]);
-  float s = m > st.m ? st.s * expf(st.m - m) : st.s, s1 = 0.0f;
+__device__ __forceinline__ void take(Stat& st, float x) {
+  const float m = fmaxf(st.m, x);
+  st = Stat{m, (m > st.m ? st.s * expf(st.m - m) : st.s) + exp_of(x - m)};
+}
+template <int N> __device__ __forceinline__ void take(Stat& st, const float2 (&v)[N]) {
+  float m = st.m, m1 = -FLT_MAX;
 #pragma unroll
   for (int j = 0; j < N; j += 2) {
-    s += exp_of(v[j] - m);
-    if (j + 1 < N) s1 += exp_of(v[j + 1] - m);
+    m = max3(m, v[j].x, v[j].y);
+    m1 = max3(m1, v[j + 1].x, v[j + 1].y);
   }
-  st = Stat{m, s + s1};
+  m = fmaxf(m, m1);
+  float2 s = make_float2(m > st.m ? st.s * expf(st.m - m) : st.s, 0.0f), s1 = both(0.0f);
+  const float2 below = both(-m);
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    s = __fadd2_rn(s, exp_of(__fadd2_rn(v[j], below)));
+    s1 = __fadd2_rn(s1, exp_of(__fadd2_rn(v[j + 1], below)));
+  }
+  s = __fadd2_rn(s, s1);
+  st = Stat{m, s.x + s.y};
 }
 
-// maximum and sum of this thread's part of a row; GROUP threads share the row
+// Maximum and sum of this thread's part of a row; GROUP threads share the row.  Four vectors of a thread are in flight while
+// it works on the four before.
 template <class T, int GROUP> __device__ __forceinline__ Stat scan(const T* x, uint32_t n, uint32_t tid) {
   constexpr int V = Vec<T>::n, UNROLL = 4;
   Stat st{-FLT_MAX, 0.0f};
   const uint32_t head = lead(x, n), vecs = (n - head) / V, tail = head + vecs * V;
-  for (uint32_t i = tid; i < head; i += GROUP) { const float one[1] = {as_float(x[i])}; take(st, one); }
-  const uint4* q = reinterpret_cast<const uint4*>(x + head);
-  uint32_t i = tid;
-  for (; i + (UNROLL - 1) * GROUP < vecs; i += UNROLL * GROUP) {
+  const uint4* q = reinterpret_cast<const uint4*>(x + head) + tid;
+  // (vectors behind the row's last are not loaded; they count as -inf)
+  uint4 ahead[UNROLL];
+  auto load = [&](uint32_t i) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (i + u * GROUP < vecs) ahead[u] = __ldg(q + (i - tid) + u * GROUP);
+  };
+  load(tid);
+  if (tid < head) take(st, as_float(x[tid]));
+  if (tail + tid < n) take(st, as_float(x[tail + tid]));
+  for (uint32_t i = tid; i < vecs; i += UNROLL * GROUP) {
     uint4 w[UNROLL];
-    float v[UNROLL * V];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) w[u] = __ldg(q + i + u * GROUP);
+    for (int u = 0; u < UNROLL; ++u) w[u] = ahead[u];
+    load(i + UNROLL * GROUP);
+    if (i + (UNROLL - 1) * GROUP < vecs) {
+      float2 v[UNROLL * V / 2];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) Vec<T>::open(w[u], reinterpret_cast<float(&)[V]>(v[u * V]));
-    take(st, v);
+      for (int u = 0; u < UNROLL; ++u) Vec<T>::open(w[u], v + u * (V / 2));
+      take(st, v);
+    } else {
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u)
+        if (i + u * GROUP < vecs) {
+          float2 v[V / 2];
+          Vec<T>::open(w[u], v);
+          take(st, v);
+        }
+    }
   }
-  for (; i < vecs; i += GROUP) {
-    float v[V];
-    Vec<T>::open(__ldg(q + i), v);
-    take(st, v);
-  }
-  for (uint32_t j = tail + tid; j < n; j += GROUP) { const float one[1] = {as_float(x[j])}; take(st, one); }
   return st;
 }
 // The group's maximum and sum, the same bits in every thread (a butterfly of plain sums is symmetric).
@@ -143,8 +187,7 @@ template <int GROUP> __device__ __forceinline__ Stat join_group(Stat st) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (GROUP > 32) {
-    __shared__ Stat part[kThreads / 32];
-    __syncthreads();                              // the last row's have been read
+    __shared__ Stat part[GROUP / 32];
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = Stat{m, s};
     __syncthreads();
 #pragma unroll
@@ -166,92 +209,128 @@ template <class T, int GROUP> __device__ __forceinline__ void clear_row(T* out, 
   for (uint32_t j = tail + tid; j < n; j += GROUP) out[j] = from_float<T>(0.0f);
 }
 // out = w (onehot - exp(x - lse)); w = 0 gives zeros unless the row holds something that is no number
-template <class T, int GROUP>
-__device__ __forceinline__ void grad_row(const T* x, T* out, uint32_t n, uint32_t label, float lse, float w, uint32_t tid) {
-  constexpr int V = Vec<T>::n;
-  auto one = [&](uint32_t i) {
-    const float p = exp_of(as_float(x[i]) - lse);
+template <class T> struct GradRow {
+  static constexpr int V = Vec<T>::n;
+  float lse, w;
+  uint32_t label;
+  __device__ __forceinline__ GradRow(float lse_, float w_, uint32_t label_) : lse(lse_), w(w_), label(label_) {}
+  __device__ __forceinline__ void one(const T* x, T* out, uint32_t i) const {
+    const float p = exp_near(as_float(x[i]) - lse);
     out[i] = from_float<T>(i == label ? __fmaf_rn(-w, p, w) : __fmul_rn(-w, p));
-  };
-  const uint32_t head = lead(x, n), vecs = (n - head) / V, tail = head + vecs * V;
+  }
+  __device__ __forceinline__ uint4 cold(const uint4& q) const {      // a vector that does not hold the label
+    const float2 below = both(-lse), minus = both(-w);
+    float2 v[V / 2];
+    Vec<T>::open(q, v);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) v[j] = __fmul2_rn(minus, exp_near(__fadd2_rn(v[j], below)));
+    return Vec<T>::close(v);
+  }
+  __device__ __forceinline__ uint4 hot(const uint4& q, uint32_t at) const {      // one that holds it, as element `at`
+    const float2 below = both(-lse), minus = both(-w);
+    float2 v[V / 2];
+    Vec<T>::open(q, v);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j)
+      v[j] = __ffma2_rn(minus, exp_near(__fadd2_rn(v[j], below)), make_float2(at == 2 * j ? w : 0.0f, at == 2 * j + 1 ? w : 0.0f));
+    return Vec<T>::close(v);
+  }
+};
+template <class T, int GROUP, int UNROLL>
+__device__ __forceinline__ void grad_row(const T* x, T* out, uint32_t n, uint32_t label, float lse, float w, uint32_t tid) {
+  const GradRow<T> g(lse, w, label);
+  const uint32_t head = lead(x, n), vecs = (n - head) / Vec<T>::n, tail = head + vecs * Vec<T>::n;
   if (lead(out, n) != head) {                     // the two rows lie differently: element by element
-    for (uint32_t i = tid; i < n; i += GROUP) one(i);
+    for (uint32_t i = tid; i < n; i += GROUP) g.one(x, out, i);
     return;
   }
-  for (uint32_t i = tid; i < head; i += GROUP) one(i);
+  if (tid < head) g.one(x, out, tid);
+  if (tail + tid < n) g.one(x, out, tail + tid);
   const uint4* q = reinterpret_cast<const uint4*>(x + head);
   uint4* o = reinterpret_cast<uint4*>(out + head);
-  const uint32_t hot = label - head;              // (wraps when the label lies in front: then no vector holds it)
-#pragma unroll 2
-  for (uint32_t i = tid; i < vecs; i += GROUP) {
-    float v[V];
-    Vec<T>::open(__ldg(q + i), v);
-    const uint32_t at = hot / V == i ? hot % V : V;
+  const uint32_t hot = (label - head) / Vec<T>::n, at = (label - head) % Vec<T>::n;     // (a label in front wraps: no vector's)
+  for (uint32_t i = tid; i < vecs; i += UNROLL * GROUP) {
+    uint4 v[UNROLL];
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = __fmaf_rn(-w, exp_of(v[j] - lse), at == j ? w : 0.0f);
-    o[i] = Vec<T>::close(v);
+    for (int u = 0; u < UNROLL; ++u)
+      if (i + u * GROUP < vecs) v[u] = __ldg(q + i + u * GROUP);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (i + u * GROUP < vecs) o[i + u * GROUP] = i + u * GROUP == hot ? g.hot(v[u], at) : g.cold(v[u]);
   }
-  for (uint32_t j = tail + tid; j < n; j += GROUP) one(j);
 }
 
 template <class T> __device__ __forceinline__ const T* row_of(const Rows& r, int64_t row) {
   const int64_t b = row / r.seq, t = row - b * r.seq;
   return static_cast<const T*>(r.x) + b * r.stride_b + t * r.stride_t;
 }
-// log-probability of a label; NaN for a label that is no index
-template <class T> __device__ __forceinline__ double logp_of(const T* x, int64_t label, uint32_t vocab, double lse) {
-  return label >= 0 && label < (int64_t)vocab ? (double)as_float(x[label]) - lse : (double)__uint_as_float(0x7fc00000u);
-}
-template <int GROUP> struct Group {               // rows are dealt to the groups of the grid in turn
-  static constexpr int per_cta = kThreads / GROUP;
-  static __device__ __forceinline__ uint32_t tid() { return GROUP == kThreads ? threadIdx.x : threadIdx.x & 31; }
-  static __device__ __forceinline__ int64_t first() {
-    return GROUP == kThreads ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * per_cta + (threadIdx.x >> 5);
+template <class T> struct Out {                   // where the gradient's rows lie
+  T* x;
+  int64_t stride_b, stride_t;
+  __device__ __forceinline__ T* row(int64_t i, uint32_t seq) const {
+    const int64_t b = i / seq, t = i - b * seq;
+    return x + b * stride_b + t * stride_t;
   }
-  static __device__ __forceinline__ int64_t step() { return (int64_t)gridDim.x * per_cta; }
+};
+// the label's logit; NaN for a label that is no index
+template <class T> __device__ __forceinline__ float at_label(const T* x, int64_t label, uint32_t vocab) {
+  return label >= 0 && label < (int64_t)vocab ? as_float(x[label]) : __uint_as_float(0x7fc00000u);
+}
+template <int GROUP> struct Group {               // a row's threads: a warp of a CTA of kThreads, or a CTA; one group for each row
+  static constexpr int threads = GROUP == 32 ? kThreads : GROUP, per_cta = threads / GROUP;
+  static __device__ __forceinline__ uint32_t tid() { return GROUP == 32 ? threadIdx.x & 31 : threadIdx.x; }
+  static __device__ __forceinline__ int64_t row() {
+    return GROUP == 32 ? (int64_t)blockIdx.x * per_cta + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+  }
 };
 
 // L: fp32 for the caller, fp64 for the preference loss, whose rewards are small differences of long sums
 template <class T, int GROUP, class L>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const Rows r, L* __restrict__ logp, float* __restrict__ lse_out,
-                                                           unsigned int* __restrict__ ticket) {
+__global__ void __launch_bounds__(Group<GROUP>::threads, 1024 / Group<GROUP>::threads)
+forward_kernel(const Rows r, L* __restrict__ logp, float* __restrict__ lse_out, unsigned int* __restrict__ ticket) {
   using G = Group<GROUP>;
   if (ticket != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;      // for the kernel behind this one
-  for (int64_t row = G::first(); row < r.rows; row += G::step()) {
-    const int64_t label = r.labels[row];
-    if (label == r.ignore) {
-      if (G::tid() == 0) { logp[row] = (L)0; lse_out[row] = 0.0f; }
-      continue;
-    }
-    const T* x = row_of<T>(r, row);
-    const Stat st = join_group<GROUP>(scan<T, GROUP>(x, r.vocab, G::tid()));
-    if (G::tid() == 0) {
-      const double lse = lse_of(st);
-      lse_out[row] = (float)lse;
-      logp[row] = (L)logp_of(x, label, r.vocab, lse);
-    }
+  const int64_t row = G::row();
+  if (row >= r.rows) return;
+  const int64_t label = r.labels[row];
+  if (label == r.ignore) {
+    if (G::tid() == 0) { logp[row] = (L)0; lse_out[row] = 0.0f; }
+    return;
+  }
+  const T* x = row_of<T>(r, row);
+  const Stat st = join_group<GROUP>(scan<T, GROUP>(x, r.vocab, G::tid()));
+  if (G::tid() == 0) {
+    const double lse = lse_of(st);
+    lse_out[row] = (float)lse;
+    logp[row] = (L)((double)at_label(x, label, r.vocab) - lse);
   }
 }
 
-// w of row i: weight[i / per] (* *scale).  unless_one: nothing is left to do when *scale is 1.
-template <class T, int GROUP>
-__global__ void __launch_bounds__(kThreads) backward_kernel(const Rows r, const float* __restrict__ lse, const float* __restrict__ weight,
-                                                            uint32_t per, const float* __restrict__ scale, bool unless_one,
-                                                            T* __restrict__ out) {
+// w of row i: weight[i / per] (* *scale).  UNLESS_ONE: nothing is left to do when *scale is 1, which is most often so: then few
+// CTAs are launched, which go through the rows in turn where they have to.
+template <class T, int GROUP, bool UNLESS_ONE>
+__global__ void __launch_bounds__(Group<GROUP>::threads) backward_kernel(const Rows r, const float* __restrict__ lse,
+                                                                         const float* __restrict__ weight, uint32_t per,
+                                                                         const float* __restrict__ scale, const Out<T> out) {
   using G = Group<GROUP>;
   const float by = scale != nullptr ? *scale : 1.0f;
-  if (unless_one && by == 1.0f) return;
-  for (int64_t i = G::first(); i < r.rows; i += G::step()) {
+  auto one = [&](int64_t i) {
     const int64_t row = r.rows - 1 - i, label = r.labels[row];
-    T* o = out + row * r.vocab;
+    T* o = out.row(row, r.seq);
     float w = label == r.ignore ? 0.0f : weight[row / per] * by;
     const float l = lse[row];
     if (label == r.ignore || (w == 0.0f && fabsf(l) <= FLT_MAX)) {
       clear_row<T, GROUP>(o, r.vocab, G::tid());
-      continue;
+      return;
     }
     if (label < 0 || label >= (int64_t)r.vocab) w = __uint_as_float(0x7fc00000u);
-    grad_row<T, GROUP>(row_of<T>(r, row), o, r.vocab, (uint32_t)label, l, w, G::tid());
+    grad_row<T, GROUP, 2>(row_of<T>(r, row), o, r.vocab, (uint32_t)label, l, w, G::tid());
+  };
+  if constexpr (UNLESS_ONE) {
+    if (by == 1.0f) return;
+    for (int64_t i = G::row(); i < r.rows; i += (int64_t)gridDim.x * G::per_cta) one(i);
+  } else if (G::row() < r.rows) {
+    one(G::row());
   }
 }
 
@@ -335,67 +414,119 @@ struct Policy {
   uint32_t per;
   float low, high, kl;      // 1 - clip, 1 + clip_high, coefficient of the KL term
 };
+// Rows that have a label: one count per CTA, which those who need it add up.  Also readies the words of the kernels behind it.
+constexpr int kCountParts = 148;
+struct Words {
+  unsigned int ticket;
+  unsigned int count[kCountParts];
+};
 __global__ void __launch_bounds__(kThreads) count_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t ignore,
-                                                         unsigned long long* __restrict__ count) {
+                                                         Words* __restrict__ words) {
   unsigned int n = 0;
+#pragma unroll 8
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rows; i += (int64_t)gridDim.x * kThreads)
     n += labels[i] != ignore;
+  __shared__ unsigned int part[kThreads / 32];
   n = __reduce_add_sync(0xffffffffu, n);
-  if ((threadIdx.x & 31) == 0 && n != 0) atomicAdd(count, (unsigned long long)n);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) n += part[w];
+    words->count[blockIdx.x] = n;
+    if (blockIdx.x == 0) words->ticket = 0;
+  }
+}
+// (the counts are loaded by the lanes of a warp, long before their sum is needed)
+__device__ __forceinline__ unsigned int my_counts(const Words* words, int parts) {
+  unsigned int n = 0;
+  for (int i = threadIdx.x & 31; i < parts; i += 32) n += words->count[i];
+  return n;
+}
+__device__ __forceinline__ float share_of(unsigned int counts) {
+  const unsigned int live = __reduce_add_sync(0xffffffffu, counts);
+  return 1.0f / (float)(live > 0 ? live : 1);
 }
 
 struct PolicyOut {
   float* logp;              // [rows]
   float* lse;               // [rows]
   float* weight;            // [rows]: dloss / dlogp
-  float* loss;
-  float* stats;             // mean of the KL term, share of clipped rows
-  double* parts;
-  unsigned int* ticket;
+  float* term;              // [2, rows]: the row's loss; its KL term, with the sign set where the clamp cut the gradient
 };
-template <class T, int GROUP>
-__global__ void __launch_bounds__(kThreads) policy_kernel(const Rows r, const Policy p, const unsigned long long* __restrict__ count,
-                                                          const PolicyOut o, T* __restrict__ grad) {
-  using G = Group<GROUP>;
-  const unsigned long long live = *count;
-  const float share = 1.0f / (float)(live > 0 ? live : 1);
-  double sum[3] = {0.0, 0.0, 0.0};
-  for (int64_t row = G::first(); row < r.rows; row += G::step()) {
-    const int64_t label = r.labels[row];
-    if (label == r.ignore) {
-      if (G::tid() == 0) { o.logp[row] = 0.0f; o.lse[row] = 0.0f; o.weight[row] = 0.0f; }
-      if (grad != nullptr) clear_row<T, GROUP>(grad + row * r.vocab, r.vocab, G::tid());
-      continue;
-    }
-    const T* x = row_of<T>(r, row);
-    const Stat st = join_group<GROUP>(scan<T, GROUP>(x, r.vocab, G::tid()));
-    const double lse64 = lse_of(st);
-    const float lse = (float)lse64, logp = (float)logp_of(x, label, r.vocab, lse64);
-    const float a = p.advantage[row / p.per], rho = expf(logp - p.old[row]);
-    const float s = rho * a, q = fminf(fmaxf(rho, p.low), p.high) * a;
-    const bool clipped = s > q;                              // (not when it is no number: that has to show)
-    float w = clipped ? 0.0f : -s, kl = 0.0f;
-    if (p.ref != nullptr) {
-      const float d = p.ref[row] - logp, e = expm1f(d);
-      kl = e - d;
-      w -= p.kl * e;
-    }
-    w *= share;
-    if (G::tid() == 0) {
-      o.logp[row] = logp;
-      o.lse[row] = lse;
-      o.weight[row] = w;
-      sum[0] += (double)(p.kl * kl) - (double)(clipped ? q : s);
-      sum[1] += (double)kl;
-      sum[2] += clipped ? 1.0 : 0.0;
-    }
-    if (grad != nullptr) grad_row<T, GROUP>(x, grad + row * r.vocab, r.vocab, (uint32_t)label, lse, w, G::tid());
+// What the loss needs of a row beside its sum, loaded while that is found.
+struct RowIn {
+  float advantage, old, ref, x;
+};
+template <class T> __device__ __forceinline__ RowIn row_in(const Policy& p, int64_t row, const T* x, int64_t label, uint32_t vocab) {
+  return RowIn{p.advantage[row / p.per], p.old[row], p.ref != nullptr ? p.ref[row] : 0.0f, at_label(x, label, vocab)};
+}
+// The row's results, stored by its first thread, and its weight.
+__device__ __forceinline__ float policy_row(const Policy& p, const PolicyOut& o, int64_t rows, int64_t row, const RowIn& in, double lse64,
+                                            float share, bool store) {
+  const float logp = (float)((double)in.x - lse64), a = in.advantage, rho = expf(logp - in.old);
+  const float s = rho * a, q = fminf(fmaxf(rho, p.low), p.high) * a;
+  const bool clipped = s > q;                                // (not when it is no number: that has to show)
+  float w = clipped ? 0.0f : -s, kl = 0.0f;
+  if (p.ref != nullptr) {
+    const float d = in.ref - logp, e = expm1f(d);
+    kl = fabsf(e - d);                                       // (never negative but for the last rounding)
+    w = fmaf(-p.kl, e, w);
   }
-  if (grid_sum(sum, o.parts, o.ticket) && threadIdx.x == 0) {
-    const double n = (double)(live > 0 ? live : 1);
-    *o.loss = (float)(sum[0] / n);
-    o.stats[0] = (float)(sum[1] / n);
-    o.stats[1] = (float)(sum[2] / n);
+  w *= share;
+  if (store) {
+    o.logp[row] = logp;
+    o.lse[row] = (float)lse64;
+    o.weight[row] = w;
+    o.term[row] = fmaf(p.kl, kl, -(clipped ? q : s));
+    o.term[rows + row] = clipped ? -kl : kl;
+  }
+  return w;
+}
+__device__ __forceinline__ void no_row(const PolicyOut& o, int64_t rows, int64_t row) {
+  o.logp[row] = o.lse[row] = o.weight[row] = o.term[row] = o.term[rows + row] = 0.0f;
+}
+
+// One group for each row, which it reads twice when it writes the gradient: the second time from L2.
+template <class T, int GROUP>
+__global__ void __launch_bounds__(Group<GROUP>::threads) policy_kernel(const Rows r, const Policy p, const Words* __restrict__ words, int parts,
+                                                                       const PolicyOut o, const Out<T> grad) {
+  using G = Group<GROUP>;
+  const int64_t row = G::row();
+  if (row >= r.rows) return;
+  const unsigned int counts = my_counts(words, parts);
+  const int64_t label = r.labels[row];
+  if (label == r.ignore) {
+    if (G::tid() == 0) no_row(o, r.rows, row);
+    if (grad.x != nullptr) clear_row<T, GROUP>(grad.row(row, r.seq), r.vocab, G::tid());
+    return;
+  }
+  const T* x = row_of<T>(r, row);
+  const RowIn in = row_in(p, row, x, label, r.vocab);
+  const Stat st = join_group<GROUP>(scan<T, GROUP>(x, r.vocab, G::tid()));
+  const double lse = lse_of(st);
+  const float w = policy_row(p, o, r.rows, row, in, lse, share_of(counts), G::tid() == 0);
+  if (grad.x != nullptr) grad_row<T, GROUP, 8>(x, grad.row(row, r.seq), r.vocab, (uint32_t)label, (float)lse, w, G::tid());
+}
+
+// Means over the rows with a label, in 64 bits and in a fixed order.
+__global__ void __launch_bounds__(kThreads) policy_sum_kernel(const float* __restrict__ term, const int64_t* __restrict__ labels, int64_t ignore,
+                                                              int64_t rows, Words* __restrict__ words, double* __restrict__ parts,
+                                                              float* __restrict__ loss, float* __restrict__ stats) {
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rows; i += (int64_t)gridDim.x * kThreads) {
+    const float kl = term[rows + i];
+    sum[0] += (double)term[i];
+    sum[1] += fabs((double)kl);
+    sum[2] += (__float_as_uint(kl) >> 31) != 0u ? 1.0 : 0.0;
+    sum[3] += labels[i] != ignore ? 1.0 : 0.0;
+  }
+  if (grid_sum(sum, parts, &words->ticket) && threadIdx.x == 0) {
+    const double n = fmax(sum[3], 1.0);
+    *loss = (float)(sum[0] / n);
+    stats[0] = (float)(sum[1] / n);
+    stats[1] = (float)(sum[2] / n);
   }
 }
 
@@ -405,35 +536,52 @@ inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintp
 int check_rows(const nvfp4_logit_rows* in, Rows& r) {
   if (in == nullptr || !in->logits || !in->labels) return NVFP4_E_NULL;
   if (in->batch <= 0 || in->seq <= 0 || in->vocab <= 0) return NVFP4_E_SHAPE;
-  if (in->seq > 0x7fffffffLL || in->vocab > 0x7fffffffLL || in->batch > INT64_MAX / in->seq / in->vocab / 4) return NVFP4_E_LIMIT;
+  if (in->seq > 0x7fffffffLL || in->vocab > 0x7fffffffLL || in->batch > INT64_MAX / in->seq / in->vocab / 4 ||
+      in->batch > 0x7fffffffLL / in->seq)
+    return NVFP4_E_LIMIT;
   if (!aligned(in->logits, in->is_f32 ? 4 : 2) || !aligned(in->labels, 8)) return NVFP4_E_ALIGN;
   r = Rows{in->logits, in->stride_b, in->stride_t, in->batch * in->seq, (uint32_t)in->seq, (uint32_t)in->vocab, in->labels,
            in->ignore_index};
   return NVFP4_OK;
 }
-// CTAs for `rows` rows in groups of a warp or a CTA: enough to fill the machine, few enough to sum their parts quickly
-unsigned grid_of(const Rows& r) {
-  const int64_t ctas = r.vocab <= kWarpRow ? (r.rows + kThreads / 32 - 1) / (kThreads / 32) : r.rows;
-  return (unsigned)(ctas < NVFP4_LOSS_PARTS ? ctas : NVFP4_LOSS_PARTS);
-}
 int launched() { return cudaGetLastError() == cudaSuccess ? NVFP4_OK : NVFP4_E_LAUNCH; }
 
-// f(type tag, group size tag)
-template <class F> void by_kind(bool f32, const Rows& r, F f) {
-  using Warp = std::integral_constant<int, 32>;
-  using Cta = std::integral_constant<int, kThreads>;
-  if (f32) {
-    if (r.vocab <= kWarpRow) f(float(), Warp());
-    else f(float(), Cta());
-  } else {
-    if (r.vocab <= kWarpRow) f(__nv_bfloat16(), Warp());
-    else f(__nv_bfloat16(), Cta());
-  }
+// f(type tag, group size tag, grid): one group for each row, a warp up to kWarpRow logits, else a CTA of LONG threads.
+template <int LONG, class F> void by_rows(bool f32, const Rows& r, F f) {
+  auto sized = [&](auto t) {
+    if (r.vocab <= kWarpRow) f(t, std::integral_constant<int, 32>(), (unsigned)((r.rows + kThreads / 32 - 1) / (kThreads / 32)));
+    else f(t, std::integral_constant<int, LONG>(), (unsigned)r.rows);
+  };
+  if (f32) sized(float());
+  else sized(__nv_bfloat16());
 }
+// Sums over long rows: eight CTAs of 128 threads an SM when there are rows for them (16384 rows of 50257 bf16: 246 us, 262 with
+// four of 256, 332 with two of 512), else 512 threads a row (231 rows of 50257 fp32: 10.0 us, 13.2, 20.6 the other way).
 template <class L> void forward(const Rows& r, bool f32, L* logp, float* lse, unsigned int* ticket, cudaStream_t stream) {
-  by_kind(f32, r, [&](auto t, auto g) {
-    forward_kernel<decltype(t), decltype(g)::value, L><<<grid_of(r), kThreads, 0, stream>>>(r, logp, lse, ticket);
-  });
+  auto go = [&](auto t, auto g, unsigned grid) {
+    constexpr int G = decltype(g)::value;
+    forward_kernel<decltype(t), G, L><<<grid, Group<G>::threads, 0, stream>>>(r, logp, lse, ticket);
+  };
+  if (r.rows >= 148 * 8) by_rows<128>(f32, r, go);
+  else by_rows<512>(f32, r, go);
+}
+
+constexpr int kWordsBytes = 1024;
+static_assert(sizeof(Words) <= kWordsBytes && kWordsBytes + 4 * 8 * NVFP4_LOSS_PARTS <= NVFP4_LOSS_WORKSPACE, "");
+
+// The row is read again right behind its sum: 256 threads a row keep so few rows under way that they stay in L2, and eight
+// vectors of a thread in flight hide its latency (8192 rows of 50257 bf16, a quarter masked: 276 us; 317 with two vectors, 285 with
+// four; with four and 512 threads 306, with 128 330; 309 with the row kept in shared memory and the next one copied in
+// behind it).  The same kernel with and without a gradient: the loss has the same bits.
+void policy_rows(const Rows& r, bool f32, const Policy& p, Words* words, int counts, const PolicyOut& o, void* dlogits, int64_t dstride_b,
+                 int64_t dstride_t, cudaStream_t stream) {
+  auto go = [&](auto t, auto g, unsigned grid) {
+    using T = decltype(t);
+    constexpr int G = decltype(g)::value;
+    policy_kernel<T, G><<<grid, Group<G>::threads, 0, stream>>>(r, p, words, counts, o, Out<T>{static_cast<T*>(dlogits), dstride_b, dstride_t});
+  };
+  if (r.rows >= 148 * 4) by_rows<256>(f32, r, go);
+  else by_rows<512>(f32, r, go);
 }
 
 }  // namespace logprob
@@ -451,16 +599,21 @@ extern "C" int nvfp4_logprob_fwd(const nvfp4_logit_rows* in, float* logp, float*
 }
 
 extern "C" int nvfp4_logprob_bwd(const nvfp4_logit_rows* in, const float* lse, const float* weight, int64_t rows_per_weight,
-                                 const float* scale, int unless_one, void* dlogits, void* stream_) {
+                                 const float* scale, int unless_one, void* dlogits, int64_t dstride_b, int64_t dstride_t,
+                                 void* stream_) {
   Rows r;
   if (const int code = check_rows(in, r); code != NVFP4_OK) return code;
   if (!lse || !weight || !dlogits || (unless_one && !scale)) return NVFP4_E_NULL;
   if (rows_per_weight <= 0 || rows_per_weight > 0x7fffffffLL) return NVFP4_E_SHAPE;
   if (!aligned(lse, 4) || !aligned(weight, 4) || !aligned(scale, 4) || !aligned(dlogits, in->is_f32 ? 4 : 2)) return NVFP4_E_ALIGN;
-  by_kind(in->is_f32 != 0, r, [&](auto t, auto g) {
+  by_rows<512>(in->is_f32 != 0, r, [&](auto t, auto g, unsigned grid) {
     using T = decltype(t);
-    backward_kernel<T, decltype(g)::value><<<grid_of(r), kThreads, 0, static_cast<cudaStream_t>(stream_)>>>(
-        r, lse, weight, (uint32_t)rows_per_weight, scale, unless_one != 0, static_cast<T*>(dlogits));
+    constexpr int G = decltype(g)::value;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    const Out<T> out{static_cast<T*>(dlogits), dstride_b, dstride_t};
+    const uint32_t per = (uint32_t)rows_per_weight;
+    if (unless_one) backward_kernel<T, G, true><<<grid < 148 * 4 ? grid : 148 * 4, Group<G>::threads, 0, stream>>>(r, lse, weight, per, scale, out);
+    else backward_kernel<T, G, false><<<grid, Group<G>::threads, 0, stream>>>(r, lse, weight, per, scale, out);
   });
   return launched();
 }
@@ -489,29 +642,31 @@ extern "C" int nvfp4_preference_fwd(const nvfp4_logit_rows* in, const float* ref
 
 extern "C" int nvfp4_policy_fwd(const nvfp4_logit_rows* in, const float* old_logp, const float* advantage,
                                 int64_t rows_per_advantage, const float* ref_logp, double clip_low, double clip_high, double kl,
-                                float* logp, float* lse, float* weight, float* loss, float* stats2, void* dlogits,
-                                void* workspace, size_t workspace_bytes, void* stream_) {
+                                float* logp, float* lse, float* weight, float* terms, float* loss, float* stats2, void* dlogits,
+                                int64_t dstride_b, int64_t dstride_t, void* workspace, size_t workspace_bytes, void* stream_) {
   Rows r;
   if (const int code = check_rows(in, r); code != NVFP4_OK) return code;
-  if (!old_logp || !advantage || !logp || !lse || !weight || !loss || !stats2 || !workspace) return NVFP4_E_NULL;
+  if (!old_logp || !advantage || !logp || !lse || !weight || !terms || !loss || !stats2 || !workspace) return NVFP4_E_NULL;
   if (rows_per_advantage <= 0 || rows_per_advantage > 0x7fffffffLL) return NVFP4_E_SHAPE;
   if (workspace_bytes < NVFP4_LOSS_WORKSPACE) return NVFP4_E_WORKSPACE;
   if (!aligned(old_logp, 4) || !aligned(advantage, 4) || !aligned(ref_logp, 4) || !aligned(logp, 4) || !aligned(lse, 4) ||
-      !aligned(weight, 4) || !aligned(loss, 4) || !aligned(stats2, 4) || !aligned(dlogits, in->is_f32 ? 4 : 2) || !aligned(workspace, 16))
+      !aligned(weight, 4) || !aligned(terms, 4) || !aligned(loss, 4) || !aligned(stats2, 4) || !aligned(dlogits, in->is_f32 ? 4 : 2) || !aligned(workspace, 16))
     return NVFP4_E_ALIGN;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  if (cudaMemsetAsync(workspace, 0, 16, stream) != cudaSuccess) return NVFP4_E_LAUNCH;
-  unsigned int* ticket = static_cast<unsigned int*>(workspace);
-  unsigned long long* count = static_cast<unsigned long long*>(workspace) + 1;
-  const int64_t ctas = (r.rows + kThreads * 4 - 1) / (kThreads * 4);
-  count_kernel<<<(unsigned)(ctas < 148 ? ctas : 148), kThreads, 0, stream>>>(r.labels, r.rows, r.ignore, count);
+  char* ws = static_cast<char*>(workspace);
+  Words* words = reinterpret_cast<Words*>(ws);
+  double* parts = reinterpret_cast<double*>(ws + kWordsBytes);
+  const int64_t ctas = (r.rows + kThreads * 8 - 1) / (kThreads * 8);
+  const int counts = (int)(ctas < kCountParts ? ctas : kCountParts);
+  count_kernel<<<counts, kThreads, 0, stream>>>(r.labels, r.rows, r.ignore, words);
   if (const int code = launched(); code != NVFP4_OK) return code;
   const Policy p{old_logp, ref_logp, advantage, (uint32_t)rows_per_advantage, (float)(1.0 - clip_low),
                  (float)(1.0 + clip_high), (float)kl};
-  const PolicyOut o{logp, lse, weight, loss, stats2, reinterpret_cast<double*>(static_cast<char*>(workspace) + 16), ticket};
-  by_kind(in->is_f32 != 0, r, [&](auto t, auto g) {
-    using T = decltype(t);
-    policy_kernel<T, decltype(g)::value><<<grid_of(r), kThreads, 0, stream>>>(r, p, count, o, static_cast<T*>(dlogits));
-  });
+  const PolicyOut o{logp, lse, weight, terms};
+  policy_rows(r, in->is_f32 != 0, p, words, counts, o, dlogits, dstride_b, dstride_t, stream);
+  if (const int code = launched(); code != NVFP4_OK) return code;
+  const int64_t sums = (r.rows + kThreads * 8 - 1) / (kThreads * 8);
+  policy_sum_kernel<<<(unsigned)(sums < NVFP4_LOSS_PARTS ? sums : NVFP4_LOSS_PARTS), kThreads, 0, stream>>>(
+      terms, r.labels, r.ignore, r.rows, words, parts, loss, stats2);
   return launched();
 }

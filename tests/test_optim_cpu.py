@@ -103,9 +103,9 @@ def test_c_entry_points_check_their_arguments(lib):
     assert fwd(Rows(**{**rows, "batch": 1 << 60})) == -8
     assert fwd(Rows(**{**rows, "logits": p + 2})) == -3
     r = Rows(**rows)
-    assert L.nvfp4_logprob_bwd(c.byref(r), p, p, 0, None, 0, p, None) == -2
-    assert L.nvfp4_logprob_bwd(c.byref(r), p, p, 1, None, 1, p, None) == -1       # nothing to compare with 1
+    assert L.nvfp4_logprob_bwd(c.byref(r), p, p, 0, None, 0, p, 15, 5, None) == -2
+    assert L.nvfp4_logprob_bwd(c.byref(r), p, p, 1, None, 1, p, 15, 5, None) == -1       # nothing to compare with 1
     pref = lambda r, ws: L.nvfp4_preference_fwd(c.byref(r), p, 0.1, 0.0, p, p, p, p, p, p, ws, None)
     assert pref(Rows(**{**rows, "batch": 3}), 1 << 20) == -2 and pref(r, 16) == -7
-    assert L.nvfp4_policy_fwd(c.byref(r), p, p, 3, None, 0.2, 0.2, 0.0, p, p, p, p, p, None, p, 16, None) == -7
-    assert L.nvfp4_policy_fwd(c.byref(r), p, p, 0, None, 0.2, 0.2, 0.0, p, p, p, p, p, None, p, 1 << 20, None) == -2
+    assert L.nvfp4_policy_fwd(c.byref(r), p, p, 3, None, 0.2, 0.2, 0.0, p, p, p, p, p, p, None, 0, 0, p, 16, None) == -7
+    assert L.nvfp4_policy_fwd(c.byref(r), p, p, 0, None, 0.2, 0.2, 0.0, p, p, p, p, p, p, None, 0, 0, p, 1 << 20, None) == -2

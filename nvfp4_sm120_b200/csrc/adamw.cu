@@ -311,10 +311,15 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constan
   }
 }
 
-__device__ __forceinline__ float root_approx(float x) {
-  float r;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
+// Roots of two numbers: the approximate reciprocal root and one Newton step with the exact residual (Markstein 1990), which gives
+// the correctly rounded root but for cases too close to call in 44 bits.  What is below 2^-120 comes out smaller than its
+// root, zero as zero: a root under 2^-60 is nothing beside any eps.
+__device__ __forceinline__ float2 roots(float2 x) {
+  float2 y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(fmaxf(x.x, 0x1p-120f)));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(fmaxf(x.y, 0x1p-120f)));
+  const float2 r = __fmul2_rn(x, y), minus_half = __fmul2_rn(y, both(-0.5f));
+  return __ffma2_rn(__ffma2_rn(r, r, make_float2(-x.x, -x.y)), minus_half, r);
 }
 __device__ __forceinline__ float reciprocal_approx(float x) {
   float r;
@@ -323,8 +328,8 @@ __device__ __forceinline__ float reciprocal_approx(float x) {
 }
 
 // The same step on 8-bit moments.  It is bound by instructions as much as by memory (75 for an element with the arithmetic
-// above, 16 or 10 bytes), so here products are fused with their sums and root and quotient are the approximate
-// instructions: 2^-22 of an update, beside moments that hold 2^-4.
+// above, 16 or 10 bytes).  The moments keep that arithmetic, so that the codes are those of its definition; in the update the
+// quotient is a product with the approximate reciprocal, and products are fused with their sums: 2^-21 of an update.
 //
 // A warp takes two blocks in a row of fp32 parameters, four of bf16, with the loads of all of them in flight before the
 // first is worked on; the table, the constants and the addresses are worked out once for them.  Two CTAs of 128 registers
@@ -350,9 +355,8 @@ __device__ __forceinline__ void step8(const Item8<T>& x, const Hyper& h, float c
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float2 g = __fmul2_rn(g8.v[j], both(c));
-    m.v[j] = __ffma2_rn(m.v[j], h.beta1, __fmul2_rn(g, h.rest1));
-    const float2 v = __ffma2_rn(__fmul2_rn(r.v[j], r.v[j]), h.beta2, __fmul2_rn(__fmul2_rn(g, h.rest2), g));
-    r.v[j] = make_float2(root_approx(v.x), root_approx(v.y));
+    m.v[j] = add2(mul2(m.v[j], h.beta1), mul2(g, h.rest1), h.one);
+    r.v[j] = roots(add2(mul2(mul2(r.v[j], r.v[j]), h.beta2), mul2(mul2(g, h.rest2), g), h.one));
     const float2 below = __ffma2_rn(r.v[j], h.inv_root, h.eps);
     const float2 ratio = __fmul2_rn(m.v[j], make_float2(reciprocal_approx(below.x), reciprocal_approx(below.y)));
     p.v[j] = __ffma2_rn(ratio, h.step, __fmul2_rn(p.v[j], h.decay));

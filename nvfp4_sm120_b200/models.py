@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import rotary
+from . import losses, rotary
 from .linear import FP4Linear, make_linear
 from .norm import rmsnorm_amax
 from .swiglu import relu2
@@ -158,6 +158,11 @@ class GPT(nn.Module):
         if targets is None:
             return logits, None
         return logits, F.cross_entropy(logits.reshape(-1, logits.shape[-1]).float(), targets.reshape(-1))
+
+    def token_logprobs(self, idx, targets, ignore_index=losses.IGNORE_INDEX):
+        """Log-probabilities of `targets` [batch, seq] after each prefix of `idx`, fp32, 0 where a target is ignored
+        (losses.token_logprobs; CUDA only)."""
+        return losses.token_logprobs(GPT.forward(self, idx)[0], targets, ignore_index)
 
     def num_params(self):
         """Non-embedding parameter count (the tied head counts once, as the embedding)."""

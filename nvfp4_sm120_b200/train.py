@@ -2,16 +2,23 @@
 
     python -m nvfp4_sm120_b200.train --steps 300 --backend fp4            # one GPU
     torchrun --nproc-per-node 8 -m nvfp4_sm120_b200.train --backend fp4   # data parallel over NCCL
+    python -m nvfp4_sm120_b200.train --optimizer adamw8 --objective preference   # 8-bit moments, pairs of sequences
 
 Model: 12 layers, d_model 768, 12 heads, MLP 4x, RMSNorm, RoPE, vocab 50257, seq 1024, 256
 sequences per optimizer step, AdamW lr 6e-4 with warm-up and cosine decay (the schedule of
 scaling/train_text.py:145-149).  Token ids are drawn Zipf(s = 1.1) over the vocabulary from seed 5:
 the OpenWebText slice the reference trained on is not available offline, so this is a stand-in with
 the same vocabulary and sequence format; the loss floor is the entropy of that distribution.
+
+--optimizer: torch (torch.optim.AdamW after clip_grad_norm_, the default), adamw or adamw8 (optim.AdamW with 32- or 8-bit
+moments, clipping inside its step).  --objective: lm (cross-entropy, the default); preference (losses.preference_loss on pairs
+of sequences that share their first half) or policy (losses.policy_loss on sequences scored by a fixed reward, advantages
+normalized over the microbatch), both against a frozen copy of the initial model.
 Every rank prints nothing; rank 0 prints one JSON line per logged step and a final summary."""
 from __future__ import annotations
 
 import argparse
+import copy
 import json
 import math
 import os
@@ -19,7 +26,8 @@ import time
 
 import torch
 
-from . import linear, parallel
+from . import linear, losses, parallel
+from .optim import AdamW
 from .models import GPT, GPTConfig
 
 
@@ -57,7 +65,11 @@ class Trainer:
 
     def __init__(self, dev, rank=0, world=1, backend="fp4", vocab=50257, dim=768, layers=12, heads=12, seq=1024,
                  global_batch=256, micro_batch=16, lr=6e-4, warmup=15, total_steps=300, all_fp4=False,
-                 overlap=True, group=None):
+                 overlap=True, group=None, optimizer="torch", objective="lm"):
+        if optimizer not in ("torch", "adamw", "adamw8"):
+            raise ValueError(f"optimizer must be torch, adamw or adamw8, got {optimizer}")
+        if objective not in ("lm", "preference", "policy"):
+            raise ValueError(f"objective must be lm, preference or policy, got {objective}")
         self.dev, self.rank, self.world, self.seq = dev, rank, world, seq
         self.lr, self.warmup, self.total_steps, self.global_batch = lr, warmup, total_steps, global_batch
         linear.set_amortize(True)                      # weights are quantized once per optimizer step
@@ -71,7 +83,14 @@ class Trainer:
             parallel.broadcast_parameters(self.model)
         parallel.seed_stochastic_rounding(1234, rank)
         self.params = [p for p in self.model.parameters()]
-        self.opt = torch.optim.AdamW(self.params, lr=lr, betas=(0.9, 0.95), weight_decay=0.1, fused=dev.type == "cuda")
+        if optimizer == "torch":
+            self.opt = torch.optim.AdamW(self.params, lr=lr, betas=(0.9, 0.95), weight_decay=0.1, fused=dev.type == "cuda")
+        else:
+            self.opt = AdamW(self.params, lr=lr, betas=(0.9, 0.95), weight_decay=0.1, max_norm=1.0,
+                             state_bits=8 if optimizer == "adamw8" else 32, seed=1234)
+        self.clips = optimizer != "torch"              # the step clips by itself
+        self.objective = objective
+        self.reference = None if objective == "lm" else copy.deepcopy(self.model).requires_grad_(False)
         self.sample, self.entropy = zipf_sampler(vocab, 1.1, 5 + rank, dev)
         per_rank = global_batch // world
         assert per_rank % micro_batch == 0 and per_rank * world == global_batch
@@ -86,21 +105,60 @@ class Trainer:
         self.opt.zero_grad(set_to_none=True)
         loss_sum = torch.zeros((), device=self.dev)
         for i in range(self.accum):
-            x, y = self.sample(self.micro_batch, self.seq)
-            with torch.autocast(self.dev.type, dtype=torch.bfloat16):
-                _, loss = self.model(x, y)
+            loss = getattr(self, "_" + self.objective)()
             if self.reducer is not None and i == self.accum - 1:
                 self.reducer.arm()                     # these gradients are final: reduce them as they appear
-            (loss / self.accum).backward()
-            loss_sum += loss.detach() / self.accum
+            loss.backward()
+            loss_sum += loss.detach()
         if self.reducer is not None:
             self.reducer.finish()
         elif self.world > 1:
             parallel.all_reduce_gradients(self.params, self.group)
-        torch.nn.utils.clip_grad_norm_(self.params, 1.0)
+        if not self.clips:
+            torch.nn.utils.clip_grad_norm_(self.params, 1.0)
         self.opt.step()
         linear.mark_step()
         return loss_sum
+
+    # ---- a microbatch's part of the step's loss ----
+    def _autocast(self):
+        return torch.autocast(self.dev.type, dtype=torch.bfloat16)
+
+    def _lm(self):
+        x, y = self.sample(self.micro_batch, self.seq)
+        with self._autocast():
+            _, loss = self.model(x, y)
+        return loss / self.accum
+
+    def _prompted(self, n_seq):
+        """Sequences, their targets and the targets with the prompt, the first half, ignored."""
+        x, y = self.sample(n_seq, self.seq)
+        answers = y.clone()
+        answers[:, :self.seq // 2] = losses.IGNORE_INDEX
+        return x, y, answers
+
+    def _preference(self):
+        pairs, half = self.micro_batch, self.seq // 2
+        x, y, answers = self._prompted(2 * pairs)
+        x[pairs:, :half + 1] = x[:pairs, :half + 1]    # a pair has one prompt; its last token is the first answer's input
+        with torch.no_grad(), self._autocast():
+            ref = self.reference.token_logprobs(x, answers).double().sum(1)
+        with self._autocast():
+            logits, _ = self.model(x)
+        loss, _, _ = losses.preference_loss(logits, answers, ref)
+        return loss / self.accum
+
+    def _policy(self):
+        x, y, answers = self._prompted(self.micro_batch)
+        reward = (y[:, self.seq // 2:] % 2 == 0).float().mean(1)
+        advantage = (reward - reward.mean()) / (reward.std(correction=0) + 1e-6)
+        with torch.no_grad(), self._autocast():
+            old, ref = self.model.token_logprobs(x, answers), self.reference.token_logprobs(x, answers)
+        with self._autocast():
+            logits, _ = self.model(x)
+        # scaled through its arguments: the gradient that the forward pass leaves is then the one the backward pass needs
+        loss, _ = losses.policy_loss(logits, answers, old, advantage / self.accum, ref, kl_coef=0.04 / self.accum)
+        return loss
 
 
 def main():
@@ -119,6 +177,8 @@ def main():
     ap.add_argument("--log-every", type=int, default=10)
     ap.add_argument("--all-fp4", action="store_true",
                     help="every linear of every block in FP4 (default: block 0 and the last block stay dense)")
+    ap.add_argument("--optimizer", default="torch", choices=["torch", "adamw", "adamw8"])
+    ap.add_argument("--objective", default="lm", choices=["lm", "preference", "policy"])
     ap.add_argument("--no-overlap", action="store_true", help="reduce the gradients after the backward pass")
     ap.add_argument("--out", default=None, help="append the JSON lines to this file too")
     a = ap.parse_args()
@@ -131,7 +191,7 @@ def main():
         import torch.distributed as dist
         dist.init_process_group("nccl", device_id=dev)
     tr = Trainer(dev, rank, world, a.backend, a.vocab, a.dim, a.layers, a.heads, a.seq, a.global_batch, a.micro_batch,
-                 a.lr, a.warmup, a.steps, a.all_fp4, not a.no_overlap)
+                 a.lr, a.warmup, a.steps, a.all_fp4, not a.no_overlap, optimizer=a.optimizer, objective=a.objective)
 
     def emit(rec):
         if rank == 0:
@@ -141,7 +201,7 @@ def main():
                 with open(a.out, "a") as f:
                     f.write(line + "\n")
 
-    emit({"event": "start", "backend": a.backend, "params_non_embedding": tr.model.num_params(), "world": world,
+    emit({"event": "start", "backend": a.backend, "optimizer": a.optimizer, "objective": a.objective, "params_non_embedding": tr.model.num_params(), "world": world,
           "tokens_per_step": a.global_batch * a.seq, "fp4_linears": len(tr.model.fp4_linears()),
           "zipf_entropy_nats": tr.entropy})
     t_start = None

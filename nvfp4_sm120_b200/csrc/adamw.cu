@@ -158,18 +158,18 @@ __device__ __forceinline__ double cta_sum(double s) {
   return s;
 }
 
-constexpr int kNormCap = 512, kNormGrid = 148 * 4;
-struct NormTable {
-  const void* grad[kNormCap];
-  int64_t n[kNormCap];
-  uint32_t start[kNormCap + 1];
-  uint8_t wide[kNormCap];
+constexpr int kNormSmall = 64, kNormLarge = 512, kNormGrid = 148 * 4;
+template <int CAP> struct NormTable {
+  const void* grad[CAP];
+  int64_t n[CAP];
+  uint32_t start[CAP + 1];
+  uint8_t wide[CAP];
   int32_t count;
 };
 
 constexpr int kNormChunk = 4 * kChunk;             // four loads of eight elements in flight in each thread
-template <class T>
-__global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ NormTable t, double* __restrict__ parts) {
+template <class T, int CAP>
+__global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ NormTable<CAP> t, double* __restrict__ parts) {
   double sum = 0.0;
   const uint32_t total = t.start[t.count];
   uint32_t c = blockIdx.x;
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, kResident8) adamw8_kernel(const __gr
 
 template <int CAP> constexpr bool fits() { return sizeof(Table<CAP>) + sizeof(Clip) + sizeof(PhiloxKeys) <= 32764; }
 constexpr int kSmall = 64, kLarge = 400;
-static_assert(fits<kLarge>() && sizeof(NormTable) + 8 <= 32764, "kernel parameters are 32764 bytes at most");
+static_assert(fits<kLarge>() && sizeof(NormTable<kNormLarge>) + 8 <= 32764, "kernel parameters are 32764 bytes at most");
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
@@ -474,6 +474,26 @@ int launch_step(const nvfp4_adamw_tensor* ts, int count, const nvfp4_adamw_hyper
   return cudaGetLastError() == cudaSuccess ? NVFP4_OK : NVFP4_E_LAUNCH;
 }
 
+// The CTAs that were launched, which is how many parts they leave.
+template <int CAP>
+int launch_sumsq(const void* const* grads, const int64_t* counts, int m, bool f32, double* parts, cudaStream_t stream) {
+  NormTable<CAP> t;
+  uint32_t chunks = 0;
+  for (int j = 0; j < m; ++j) {
+    t.grad[j] = grads[j];
+    t.n[j] = counts[j];
+    t.wide[j] = aligned(grads[j], f32 ? 32 : 16);
+    t.start[j] = chunks;
+    chunks += (uint32_t)((counts[j] + kNormChunk - 1) / kNormChunk);
+  }
+  t.start[m] = chunks;
+  t.count = m;
+  const int grid = chunks < kNormGrid ? (int)chunks : kNormGrid;
+  if (f32) sumsq_kernel<float, CAP><<<grid, kThreads, 0, stream>>>(t, parts);
+  else sumsq_kernel<__nv_bfloat16, CAP><<<grid, kThreads, 0, stream>>>(t, parts);
+  return grid;
+}
+
 }  // namespace adamw
 }  // namespace nvfp4
 
@@ -482,9 +502,9 @@ using namespace nvfp4::adamw;
 extern "C" int nvfp4_sumsq_parts(int count, const int64_t* counts) {
   if (count < 0 || (count > 0 && counts == nullptr)) return NVFP4_E_NULL;
   int parts = 0;
-  for (int i = 0; i < count; i += kNormCap) {
+  for (int i = 0; i < count; i += kNormLarge) {
     uint64_t chunks = 0;
-    for (int j = i; j < count && j < i + kNormCap; ++j) {
+    for (int j = i; j < count && j < i + kNormLarge; ++j) {
       if (counts[j] <= 0) return NVFP4_E_SHAPE;
       chunks += (uint64_t)((counts[j] + kNormChunk - 1) / kNormChunk);
     }
@@ -505,22 +525,10 @@ extern "C" int nvfp4_sumsq(const void* const* grads, const int64_t* counts, int 
     if (!aligned(grads[i], is_f32 ? 4 : 2)) return NVFP4_E_ALIGN;
   }
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  for (int i = 0; i < count; i += kNormCap) {
-    const int m = count - i < kNormCap ? count - i : kNormCap;
-    NormTable t;
-    uint32_t chunks = 0;
-    for (int j = 0; j < m; ++j) {
-      t.grad[j] = grads[i + j];
-      t.n[j] = counts[i + j];
-      t.wide[j] = aligned(grads[i + j], is_f32 ? 32 : 16);
-      t.start[j] = chunks;
-      chunks += (uint32_t)((counts[i + j] + kNormChunk - 1) / kNormChunk);
-    }
-    t.start[m] = chunks;
-    t.count = m;
-    const unsigned grid = chunks < kNormGrid ? chunks : kNormGrid;
-    if (is_f32) sumsq_kernel<float><<<grid, kThreads, 0, stream>>>(t, parts);
-    else sumsq_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(t, parts);
+  for (int i = 0; i < count; i += kNormLarge) {
+    const int m = count - i < kNormLarge ? count - i : kNormLarge;
+    const int grid = m <= kNormSmall ? launch_sumsq<kNormSmall>(grads + i, counts + i, m, is_f32 != 0, parts, stream)
+                                     : launch_sumsq<kNormLarge>(grads + i, counts + i, m, is_f32 != 0, parts, stream);
     if (cudaGetLastError() != cudaSuccess) return NVFP4_E_LAUNCH;
     parts += grid;
   }

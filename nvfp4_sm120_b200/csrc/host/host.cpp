@@ -355,6 +355,7 @@ const at::Tensor& tensor_of(PyObject* o) {
 }
 bool same_layout(const at::Tensor& a, const at::Tensor& b) {
   if (a.sizes() != b.sizes()) return false;
+  if (a.is_contiguous() && b.is_contiguous()) return true;
   for (int64_t d = 0; d < a.dim(); ++d)
     if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
   return true;

@@ -409,3 +409,51 @@ def test_argument_checks(losses):
     (g,) = torch.autograd.grad(lp.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):                    # no second derivative
         g.sum().backward()
+
+
+def test_more_logits_than_32_bits_count(losses):
+    rows, vocab = 42800, 50257                           # 2^31 + 3.5 million
+    assert rows * vocab > 2 ** 31
+    x = torch.zeros(rows, vocab, dtype=torch.bfloat16, device="cuda")
+    some = torch.tensor([0, 17, rows // 2, rows - 2, rows - 1], device="cuda")
+    x[some] = _logits((5, vocab), torch.bfloat16, 7)
+    x.requires_grad_(True)
+    y = torch.full((rows,), IGNORE, device="cuda")
+    y[some] = torch.tensor([0, 5, vocab - 1, 9, vocab - 1], device="cuda")
+    lp = losses.token_logprobs(x, y)
+    part = x.detach()[some]
+    _check_logp(lp.detach()[some], part, y[some])
+    w = torch.randn(rows, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    (g,) = torch.autograd.grad(lp, x, w)
+    _check_grad(g[some], part, y[some], w[some])
+    assert torch.count_nonzero(g[1:17]) == 0 and torch.count_nonzero(g[rows - 100:rows - 2]) == 0
+
+
+def test_gradients_lie_as_their_logits_do(losses):
+    """Shifted and offset views: the gradient has the view's strides, its neighbours in memory belong to nobody."""
+    base = _logits((3, 8, 2051), torch.bfloat16, 3)
+    for x in (base[:, :-1], base[:, 1:], base[:, :, 1:], base[:1, :, :7], base[:, :1], base.transpose(0, 1)):
+        x = x.detach().requires_grad_(True)
+        y = _labels(x.shape[:-1], x.shape[-1], 5)
+        w = _logits(y.shape, torch.float32, 6)
+        (g,) = torch.autograd.grad(losses.token_logprobs(x, y), x, w)
+        _check_grad(g, x.detach(), y, w)
+        c = x.detach().contiguous().requires_grad_(True)
+        (h,) = torch.autograd.grad(losses.token_logprobs(c, y), c, w)
+        assert torch.allclose(g.float(), h.float(), rtol=2.0 ** -7, atol=1e-30)
+    # through the view, into the whole tensor
+    base = base.requires_grad_(True)
+    y = _labels((3, 7), 2051, 5)
+    losses.token_logprobs(base[:, :-1], y).sum().backward()
+    assert torch.count_nonzero(base.grad[:, -1]) == 0 and torch.isfinite(base.grad).all()
+
+
+def test_inference_mode(losses):
+    with torch.inference_mode():
+        x, y = _logits((2, 3, 50), torch.float32, 1), _labels((2, 3), 50, 2, 0.0)
+        lp = losses.token_logprobs(x, y)
+        loss, chosen, _ = losses.preference_loss(x, y, lp.sum(1))
+        # the sums in fp32 here, in 64 bits there: three roundings of some ten
+        assert abs(loss.item() - math.log(2)) <= 1e-5 and abs(chosen.item()) <= 1e-5
+        loss, stats = losses.policy_loss(x, y, lp, torch.ones(2, device="cuda"))
+        assert abs(loss.item() + 1) <= 4 * U and stats["clip_fraction"].item() == 0.0

@@ -444,3 +444,22 @@ def test_refusals(optim):
         finally:
             graph.capture_end()
     assert torch.equal(p.detach(), w)
+
+
+def test_more_elements_than_32_bits_count(optim):
+    n = 2 ** 31 + 300
+    p = torch.nn.Parameter(torch.ones(n, dtype=torch.bfloat16, device="cuda"))
+    p.grad = torch.zeros_like(p)
+    ends = torch.tensor([0, 255, 256, n // 2, n - 301, n - 45, n - 1], device="cuda")
+    p.grad[ends] = 2.0
+    opt = optim.AdamW([p], lr=0.5, weight_decay=0.0, state_bits=8, max_norm=1e9)
+    opt.step()
+    # sign of the gradient at the first step, within the roundings of the update and of bf16 (0.5 is a bf16 number)
+    assert ((p.detach()[ends].float() - 0.5).abs() <= 2.0 ** -8).all()
+    assert int((p.detach() != 1).sum()) == len(ends)
+    assert abs(float(opt.grad_norm) - 2 * math.sqrt(len(ends))) <= 1e-6 * 2 * math.sqrt(len(ends))
+    st = opt.state[p]
+    codes = st["exp_avg"].view(torch.uint8)
+    assert int((codes != 0).sum()) == len(ends) and codes.numel() == -(-n // BLOCK) * BLOCK
+    del p, opt, st, codes
+    torch.cuda.empty_cache()

@@ -373,14 +373,14 @@ int nvfp4_rotary_bf16(const void* q, void* q_out, int q_heads, const void* k, vo
 
 /*
  * AdamW over many tensors at once.  For every tensor, with t its number of steps, all in fp32, every product, sum, quotient
- * and root rounded by itself:
+ * and root rounded by itself (but for p' with 8-bit moments: within 2^-21 of the update):
  *   g' = c g;  m' = b1 m + (1 - b1) g';  v' = b2 v + ((1 - b2) g') g'
  *   p' = p (1 - lr wd) - (lr / (1 - b1^t)) (m' / (sqrt(v') / sqrt(1 - b2^t) + eps))
  * param and grad are both fp32 (is_f32 != 0) or both bf16, contiguous, n elements each.
  *   state_bits 32: first = m, second = v, fp32 [n]; the scales are not looked at.
  *   state_bits 8:  first and second hold m and sqrt(v) as E4M3 codes [ceil(n / 256) * 256], first_scale and second_scale one
  *     E8M0 power of two per 256 codes [ceil(n / 256)] (byte 255: the block is NaN, which is what a block with an element
- *     of 2^51 or more, an infinity or a NaN becomes).  All zero is a valid start.  Codes are rounded stochastically: Philox4x32-10 with
+ *     of 2^51 or more, an infinity or a NaN becomes; roots under 2^-60 may come out smaller).  All zero is a valid start.  Codes are rounded stochastically: Philox4x32-10 with
  *     key philox_seed and counter (counter_base + element / 8, philox_offset), 16 bits for each of eight elements in
  *     order, low half of a word first; sqrt(v) takes the same 16 bits reversed.
  * Clipping: c = min(1, max_norm / (norm + 1e-6)) with norm from `sumsq_parts` (n_parts doubles that nvfp4_sumsq left) or

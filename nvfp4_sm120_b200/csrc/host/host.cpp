@@ -665,7 +665,7 @@ at::Tensor gradient_like(const at::Tensor& x, const Logits& in) {
 int64_t batch_stride(const at::Tensor& t) { return t.dim() == 3 ? t.stride(0) : 0; }
 
 // Nodes of the autograd graph.  In C++ because of the backward pass, which autograd runs on a thread of its own: a Python
-// node has to wait there for the interpreter lock (a loss of 48 logit rows and its gradient: 122 us, 68 us from here).
+// node has to wait there for the interpreter lock (a loss of 48 logit rows and its gradient: 122 us, 69 from here).
 using torch::autograd::AutogradContext;
 using torch::autograd::tensor_list;
 

@@ -12,7 +12,7 @@
 // A row of logits is read once with a running maximum and sum per thread, the group's are joined at the end: fp32, base
 // 2, the maximum subtracted before the product with log2 e, so that rows of the type's lowest value give no infinity.
 // The maximum starts at the lowest finite number, not at -inf: a row of -inf then ends with a sum of 0 and lse = -inf.
-// A row of more than kWarpRow logits belongs to a CTA, a shorter one to a warp.
+// A row belongs to a warp or to a CTA of 128 to 512 threads, by its length and the number of rows (group_of).
 // The policy loss's w depends on its own row alone, so its kernel writes the row's gradient right behind the sum, while
 // the row is in L2: HBM sees each row once.  The preference loss has to see both sequences first; its backward takes the
 // rows in the opposite order, so that the last ones read are still in L2.
@@ -26,7 +26,6 @@ namespace nvfp4 {
 namespace logprob {
 
 constexpr int kThreads = 256;                     // of the CTAs whose rows belong to warps, and of those that add up
-constexpr int kWarpRow = 2048;
 // log2 e in two parts: alone, the first is off by 1.3e-8 of itself, which moves every term of a row the same way, and the sum
 // of a sequence's thousand log-probabilities shows it.  (The mean error of a row's logsumexp, measured over 2048 rows of 13
 // to 50257 logits, is 1e-8; the 5e-8 by which ex2.approx falls short on average reaches the small terms only.)
@@ -306,6 +305,7 @@ forward_kernel(const Rows r, L* __restrict__ logp, float* __restrict__ lse_out, 
   }
 }
 
+// 8192 rows of 50257 bf16, half masked: 208 to 216 us, 6.1 TB/s.
 // w of row i: weight[i / per] (* *scale).  UNLESS_ONE: nothing is left to do when *scale is 1, which is most often so: then few
 // CTAs are launched, which go through the rows in turn where they have to.
 template <class T, int GROUP, bool UNLESS_ONE>
@@ -546,42 +546,56 @@ int check_rows(const nvfp4_logit_rows* in, Rows& r) {
 }
 int launched() { return cudaGetLastError() == cudaSuccess ? NVFP4_OK : NVFP4_E_LAUNCH; }
 
-// f(type tag, group size tag, grid): one group for each row, a warp up to kWarpRow logits, else a CTA of LONG threads.
-template <int LONG, class F> void by_rows(bool f32, const Rows& r, F f) {
+// Threads for a row of `vecs` 16-byte vectors.  Many short rows go to warps (16384 rows of 512 vectors, bf16, forward 34 us; 42 with
+// CTAs of 128, 167 with 512), long ones to as few threads as still have many loads in flight: the fewer, the more rows an SM has
+// under way, whose ends do not meet (16384 rows of 8192 vectors, forward 327 us with 128 threads, 415 with 512).  Kernels that
+// write read a row again behind its sum and want few of them, so that it is still in L2: more threads for long rows
+// (4096 vectors 392 us with 256 threads, 438 with 128, 478 with 512; fp32, 8192 vectors 697 with 512, 904 with 256).  Where there are few rows,
+// latency counts, and they are spread wider (16 rows of 16384 vectors, gradient: 100 us with a warp, 28 with 128 threads, 10.7 with 512).
+// Over 16 to 16384 rows of 64 to 32768 vectors no choice takes 1.35 times the best of the four.
+int group_of(int64_t rows, int64_t vecs, bool writes) {
+  if (rows >= 148 * 4) {
+    if (vecs <= 256 || (rows >= 4096 && vecs <= 1024)) return 32;
+    if (!writes || vecs <= 2048) return 128;
+    return vecs < 8192 ? 256 : 512;
+  }
+  if (vecs <= 128) return 32;
+  if (vecs <= 512) return 128;
+  return vecs <= (writes ? 2048 : 8192) ? 256 : 512;
+}
+// f(type tag, group size tag, grid)
+template <class F> void by_rows(bool f32, const Rows& r, bool writes, F f) {
+  const int group = group_of(r.rows, ((int64_t)r.vocab * (f32 ? 4 : 2) + 15) / 16, writes);
   auto sized = [&](auto t) {
-    if (r.vocab <= kWarpRow) f(t, std::integral_constant<int, 32>(), (unsigned)((r.rows + kThreads / 32 - 1) / (kThreads / 32)));
-    else f(t, std::integral_constant<int, LONG>(), (unsigned)r.rows);
+    if (group == 32) f(t, std::integral_constant<int, 32>(), (unsigned)((r.rows + kThreads / 32 - 1) / (kThreads / 32)));
+    else if (group == 128) f(t, std::integral_constant<int, 128>(), (unsigned)r.rows);
+    else if (group == 256) f(t, std::integral_constant<int, 256>(), (unsigned)r.rows);
+    else f(t, std::integral_constant<int, 512>(), (unsigned)r.rows);
   };
   if (f32) sized(float());
   else sized(__nv_bfloat16());
 }
-// Sums over long rows: eight CTAs of 128 threads an SM when there are rows for them (16384 rows of 50257 bf16: 246 us, 262 with
-// four of 256, 332 with two of 512), else 512 threads a row (231 rows of 50257 fp32: 10.0 us, 13.2, 20.6 the other way).
+// (16384 rows of 50257 bf16: 246 us, 6.7 TB/s, with eight CTAs of 128 threads an SM; 262 with four of 256)
 template <class L> void forward(const Rows& r, bool f32, L* logp, float* lse, unsigned int* ticket, cudaStream_t stream) {
-  auto go = [&](auto t, auto g, unsigned grid) {
+  by_rows(f32, r, false, [&](auto t, auto g, unsigned grid) {
     constexpr int G = decltype(g)::value;
     forward_kernel<decltype(t), G, L><<<grid, Group<G>::threads, 0, stream>>>(r, logp, lse, ticket);
-  };
-  if (r.rows >= 148 * 8) by_rows<128>(f32, r, go);
-  else by_rows<512>(f32, r, go);
+  });
 }
 
 constexpr int kWordsBytes = 1024;
 static_assert(sizeof(Words) <= kWordsBytes && kWordsBytes + 4 * 8 * NVFP4_LOSS_PARTS <= NVFP4_LOSS_WORKSPACE, "");
 
-// The row is read again right behind its sum: 256 threads a row keep so few rows under way that they stay in L2, and eight
-// vectors of a thread in flight hide its latency (8192 rows of 50257 bf16, a quarter masked: 276 us; 317 with two vectors, 285 with
-// four; with four and 512 threads 306, with 128 330; 309 with the row kept in shared memory and the next one copied in
-// behind it).  The same kernel with and without a gradient: the loss has the same bits.
+// The row is read again right behind its sum, from L2, with eight vectors of a thread in flight to hide its latency (8192 rows of
+// 50257 bf16, a quarter masked: 276 us, 5.1 TB/s; 317 with two vectors, 285 with four; 309 with the row kept in shared memory and
+// the next one copied in behind it).  The same kernel with and without a gradient: the loss has the same bits.
 void policy_rows(const Rows& r, bool f32, const Policy& p, Words* words, int counts, const PolicyOut& o, void* dlogits, int64_t dstride_b,
                  int64_t dstride_t, cudaStream_t stream) {
-  auto go = [&](auto t, auto g, unsigned grid) {
+  by_rows(f32, r, true, [&](auto t, auto g, unsigned grid) {
     using T = decltype(t);
     constexpr int G = decltype(g)::value;
     policy_kernel<T, G><<<grid, Group<G>::threads, 0, stream>>>(r, p, words, counts, o, Out<T>{static_cast<T*>(dlogits), dstride_b, dstride_t});
-  };
-  if (r.rows >= 148 * 4) by_rows<256>(f32, r, go);
-  else by_rows<512>(f32, r, go);
+  });
 }
 
 }  // namespace logprob
@@ -606,7 +620,7 @@ extern "C" int nvfp4_logprob_bwd(const nvfp4_logit_rows* in, const float* lse, c
   if (!lse || !weight || !dlogits || (unless_one && !scale)) return NVFP4_E_NULL;
   if (rows_per_weight <= 0 || rows_per_weight > 0x7fffffffLL) return NVFP4_E_SHAPE;
   if (!aligned(lse, 4) || !aligned(weight, 4) || !aligned(scale, 4) || !aligned(dlogits, in->is_f32 ? 4 : 2)) return NVFP4_E_ALIGN;
-  by_rows<512>(in->is_f32 != 0, r, [&](auto t, auto g, unsigned grid) {
+  by_rows(in->is_f32 != 0, r, true, [&](auto t, auto g, unsigned grid) {
     using T = decltype(t);
     constexpr int G = decltype(g)::value;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);

@@ -12,6 +12,7 @@
 #include <unordered_map>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -469,9 +470,9 @@ void check_state(const at::Tensor& t, c10::Device dev, at::ScalarType type, int6
     raise(PyExc_ValueError, std::string("optimizer state '") + name + "' does not fit its parameter");
 }
 
-// One step of every parameter that has a gradient.  groups: the optimizer's param_groups; state: its state.  Returns False,
-// with nothing done, when a parameter has no state yet; None when no parameter has a gradient; else the norm of all
-// gradients (0-dim) if max_norm is given, or True.
+// One step of every parameter that has a gradient.  groups: the optimizer's param_groups; state: its state.  Returns, with
+// nothing done, "state" when a parameter has no state yet and "capture" when the stream is being captured; None when no
+// parameter has a gradient; else the norm of all gradients (0-dim) if max_norm is given, or True.
 py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c10::optional<double> max_norm, uint64_t seed,
                       const OptTensor& norm_in) {
   struct Hyper {
@@ -493,7 +494,7 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
   const bool eight = bits == 8;
   static const Name kBetas("betas"), kLr("lr"), kEps("eps"), kDecay("weight_decay"), kParams("params"), kStep("step"),
       kFirst("exp_avg"), kSecond("exp_avg_sq"), kRoot("exp_avg_root"), kFirstScale("exp_avg_scale"),
-      kRootScale("exp_avg_root_scale");
+      kRootScale("exp_avg_root_scale"), kLayout("layout");
   const at::NoGradGuard no_grad;
   InOrder states{state.ptr()};
   for (py::handle gh : groups) {
@@ -512,7 +513,7 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
       check_param(p, dev);
       at::Tensor g = grad_like(p, g0);
       PyObject* st = states.find(ph.ptr());
-      if (st == nullptr) return py::bool_(false);
+      if (st == nullptr) return py::str("state");
       if (!PyDict_Check(st)) raise(PyExc_TypeError, "optimizer state holds dicts");
       Item it{};
       it.t.param = p.data_ptr();
@@ -536,6 +537,8 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
         check_state(vs, *dev, at::kFloat8_e8m0fnu, blocks, "exp_avg_root_scale");
         if (!m.is_contiguous() || !v.is_contiguous() || !ms.is_contiguous() || !vs.is_contiguous())
           raise(PyExc_ValueError, "optimizer state must be contiguous");
+        if (!same_layout(p, tensor_of(item(st, kLayout))))
+          raise(PyExc_ValueError, "a parameter's shape or strides changed: its 8-bit moments lie in the order of the old ones");
         it.t.first_scale = ms.data_ptr();
         it.t.second_scale = vs.data_ptr();
       } else {
@@ -553,6 +556,7 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
   }
   if (items.empty()) return py::none();
   const c10::cuda::CUDAGuard guard(*dev);
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return py::str("capture");
   at::Tensor parts, norm;
   const double* parts_p = nullptr;
   const float* norm_p = nullptr;

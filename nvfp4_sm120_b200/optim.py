@@ -31,7 +31,7 @@ class AdamW(torch.optim.Optimizer):
     state_bits: 32 keeps `exp_avg` and `exp_avg_sq` in fp32 (also for bf16 parameters), under torch's names, and loads
         the state_dict of a torch.optim.AdamW.  8 keeps the first moment and the ROOT of the second as E4M3 codes
         with one power of two per 256 elements (`exp_avg`, `exp_avg_scale`, `exp_avg_root`, `exp_avg_root_scale`; value =
-        code * scale, elements in memory order), rounded stochastically.  A block that holds an infinity, a NaN or a
+        code * scale, elements in memory order, which `layout` keeps), rounded stochastically.  A block that holds an infinity, a NaN or a
         magnitude of 2^51 or more is NaN as a whole from then on.
     max_norm: clip the gradients to this norm over ALL parameter groups, as clip_grad_norm_ in front of the step would,
         but inside it: `p.grad` itself is left as it is.  The norm of the last step is in `grad_norm` (0-dim, on the
@@ -81,6 +81,8 @@ class AdamW(torch.optim.Optimizer):
         at = 0
         for p, b in zip(params, blocks):
             st = {"step": 0}
+            if self.state_bits == 8:                   # (the codes follow the parameter's memory, which must not be reordered)
+                st["layout"] = torch.empty_strided(p.shape, p.stride(), device="meta")
             for name, buf in flat.items():
                 if name.endswith("_scale"):
                     st[name] = buf[at:at + b]
@@ -115,6 +117,8 @@ class AdamW(torch.optim.Optimizer):
             for st, p in pairs:
                 mine = self.state[p]
                 mine["step"] = int(st["step"])
+                if "layout" in st and (st["layout"].shape, st["layout"].stride()) != (p.shape, p.stride()):
+                    raise ValueError(f"the saved moments are in the order of strides {st['layout'].stride()}, not {p.stride()}")
                 for n in names:
                     if st[n].numel() != mine[n].numel() or (self.state_bits == 8 and st[n].dtype != mine[n].dtype):
                         raise ValueError(f"the saved {n} does not fit a parameter of shape {tuple(p.shape)}")
@@ -133,15 +137,15 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         if grad_norm is not None and self.max_norm is None:
             raise ValueError("grad_norm is what max_norm clips by: the optimizer was made without max_norm")
-        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
-            raise _lib.NVFP4Error("AdamW.step cannot be captured into a CUDA graph: its step count lives on the host")
         call = lambda: _lib.host().adamw_step(self.param_groups, self.state, self.state_bits, self.max_norm,
                                               self.seed & _M64, grad_norm)
         done = call()
-        if done is False:
+        if isinstance(done, str) and done == "state":
             for g in self.param_groups:
                 self._make_state([p for p in g["params"]
                                   if p not in self.state and p.numel() and (p.requires_grad or p.grad is not None)])
             done = call()
+        if isinstance(done, str):
+            raise _lib.NVFP4Error("AdamW.step cannot be captured into a CUDA graph: its step count lives on the host")
         self.grad_norm = done if isinstance(done, torch.Tensor) else None
         return loss

@@ -457,3 +457,22 @@ def test_inference_mode(losses):
         assert abs(loss.item() - math.log(2)) <= 1e-5 and abs(chosen.item()) <= 1e-5
         loss, stats = losses.policy_loss(x, y, lp, torch.ones(2, device="cuda"))
         assert abs(loss.item() + 1) <= 4 * U and stats["clip_fraction"].item() == 0.0
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(4100, 7001, torch.bfloat16), (600, 7001, torch.bfloat16), (600, 20011, torch.bfloat16),
+                                              (600, 40009, torch.float32), (30, 5003, torch.bfloat16), (30, 40009, torch.float32)])
+def test_every_number_of_threads_a_row(losses, rows, vocab, dtype):
+    """Warps, and CTAs of 128, 256 and 512 threads, for many rows and for few."""
+    x, y = _logits((rows, vocab), dtype, rows), _labels((rows,), vocab, 3)
+    lp64, _ = _reference(x, y)
+    w = torch.randn(rows, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4))
+    x.requires_grad_(True)
+    lp = losses.token_logprobs(x, y)
+    _check_logp(lp.detach(), x.detach(), y)
+    _check_grad(torch.autograd.grad(lp, x, w)[0], x.detach(), y, w)
+    # a policy loss whose ratios are 1.1: w = -1.1 A / n, with the error of the exponent on top
+    loss, stats = losses.policy_loss(x, y, (lp64 - math.log(1.1)).float(), w)
+    _check_logp(stats["logps"], x.detach(), y)
+    n = int((y != IGNORE).sum())
+    off = float(_lse_error(x.detach()).max()) * 1.5 + 4 * U * (float(lp64.abs().max()) + 4)
+    _check_grad(torch.autograd.grad(loss, x)[0], x.detach(), y, -1.1 * w / n, off)

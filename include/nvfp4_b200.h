@@ -380,9 +380,10 @@ int nvfp4_rotary_bf16(const void* q, void* q_out, int q_heads, const void* k, vo
  *   state_bits 32: first = m, second = v, fp32 [n]; the scales are not looked at.
  *   state_bits 8:  first and second hold m and sqrt(v) as E4M3 codes [ceil(n / 256) * 256], first_scale and second_scale one
  *     E8M0 power of two per 256 codes [ceil(n / 256)] (byte 255: the block is NaN, which is what a block with an element
- *     of 2^51 or more, an infinity or a NaN becomes; roots under 2^-60 may come out smaller).  All zero is a valid start.  Codes are rounded stochastically: Philox4x32-10 with
- *     key philox_seed and counter (counter_base + element / 8, philox_offset), 16 bits for each of eight elements in
- *     order, low half of a word first; sqrt(v) takes the same 16 bits reversed.
+ *     of 2^51 or more, an infinity or a NaN becomes; roots under 2^-60 may come out smaller).  All zero is a valid start.
+ *     Codes are rounded stochastically: Philox4x32-10 with key philox_seed and counter (counter_base + element / 8,
+ *     philox_offset), 16 bits for each of eight elements in order, low half of a word first; sqrt(v) takes the same 16
+ *     bits reversed.
  * Clipping: c = min(1, max_norm / (norm + 1e-6)) with norm from `sumsq_parts` (n_parts doubles that nvfp4_sumsq left) or
  * from the device word `norm`; c = 1 when both are NULL.  norm_out, if not NULL, receives the norm.
  * `tensors` and `hypers` are HOST arrays, read before the call returns; up to 8 hypers, which tensors name by index.
@@ -425,7 +426,8 @@ int nvfp4_norm_of_sumsq(const double* parts, int n_parts, float* norm, void* str
 /*
  * Losses on logits [batch, seq, vocab] (fp32, or bf16 when is_f32 == 0; strides in elements, the logits of a row contiguous;
  * rows are numbered batch * seq + position).  A row whose label equals ignore_index has no part in anything and is not read;
- * any other label outside [0, vocab) gives NaN.  At most 2^31 - 1 rows of at most 2^31 - 1 logits.  All row and sequence vectors are fp32.
+ * any other label outside [0, vocab) gives NaN.  At most 2^31 - 1 rows of at most 2^31 - 1 logits.  All row and sequence
+ * vectors are fp32.
  */
 typedef struct {
   const void* logits;
@@ -452,8 +454,8 @@ int nvfp4_logprob_bwd(const nvfp4_logit_rows* rows, const float* lse, const floa
                       void* stream);
 
 /*
- * Preference loss of batch / 2 pairs, sequence i chosen over sequence batch / 2 + i: with L_i the sum of the sequence's logp (fp64 here,
- * [batch * seq]: a reward is a small difference of long sums),
+ * Preference loss of batch / 2 pairs, sequence i chosen over sequence batch / 2 + i: with L_i the sum of the sequence's
+ * logp (fp64 here, [batch * seq]: a reward is a small difference of long sums),
  * rewards[i] = beta (L_i - ref[i]), h = rewards[chosen] - rewards[rejected],
  * loss = mean(-(1 - label_smoothing) logsigmoid(h) - label_smoothing logsigmoid(-h)).
  * weight[i] = dloss / dL_i, for nvfp4_logprob_bwd with rows_per_weight = seq.  No counterpart in the reference.

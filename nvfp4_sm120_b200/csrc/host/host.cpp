@@ -361,6 +361,16 @@ bool same_layout(const at::Tensor& a, const at::Tensor& b) {
     if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
   return true;
 }
+// Is `strides` (a tuple) the tensor's, where they matter?
+bool has_strides(const at::Tensor& t, PyObject* strides) {
+  if (!PyTuple_Check(strides) || PyTuple_GET_SIZE(strides) != t.dim()) return false;
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    const int64_t s = PyLong_AsLongLong(PyTuple_GET_ITEM(strides, d));
+    if (s == -1 && PyErr_Occurred()) throw py::error_already_set();
+    if (t.size(d) > 1 && s != t.stride(d)) return false;
+  }
+  return true;
+}
 // fp32 and bf16 tensors whose elements fill one piece of memory: the kernels go through it in its own order
 void check_param(const at::Tensor& p, c10::optional<c10::Device>& dev) {
   if (!p.is_cuda() || (dev.has_value() && *dev != p.device())) {
@@ -537,7 +547,7 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
         check_state(vs, *dev, at::kFloat8_e8m0fnu, blocks, "exp_avg_root_scale");
         if (!m.is_contiguous() || !v.is_contiguous() || !ms.is_contiguous() || !vs.is_contiguous())
           raise(PyExc_ValueError, "optimizer state must be contiguous");
-        if (!same_layout(p, tensor_of(item(st, kLayout))))
+        if (!has_strides(p, item(st, kLayout)))
           raise(PyExc_ValueError, "a parameter's shape or strides changed: its 8-bit moments lie in the order of the old ones");
         it.t.first_scale = ms.data_ptr();
         it.t.second_scale = vs.data_ptr();

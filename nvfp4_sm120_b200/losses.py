@@ -4,8 +4,9 @@ preference loss over pairs of sequences and a clipped policy loss with a KL term
 All take logits [batch, seq, vocab] (or [rows, vocab]; fp32 or bf16, any strides with contiguous rows) and integer labels of
 the leading shape, already shifted: labels[b, t] is the token that logits[b, t] predict, as in models.GPT.forward(idx,
 targets).  A position whose label is `ignore_index` (prompt, padding) has no part in the result and is not read; any other
-label outside the vocabulary gives NaN.  Empty logits are refused.  Arithmetic is fp32, sums over tokens are 64 bits, the gradient is rounded once to
-the logits' dtype.  Gradients are those of the logits: every other argument is a constant.  Differentiable once.
+label outside the vocabulary gives NaN.  Empty logits are refused.  Arithmetic is fp32, sums over tokens are 64 bits, the
+gradient is rounded once to the logits' dtype.  Gradients are those of the logits: every other argument is a constant.
+Differentiable once.
 
 The reference trains with cross-entropy alone (nvfp4_train.py:159-185)."""
 from __future__ import annotations

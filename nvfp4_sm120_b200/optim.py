@@ -15,6 +15,10 @@ _M64 = 2 ** 64 - 1
 _NAMES = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_scale", "exp_avg_root", "exp_avg_root_scale")}
 
 
+def _dtype8(name):
+    return torch.float8_e8m0fnu if name.endswith("_scale") else torch.float8_e4m3fn
+
+
 def grad_norm(params):
     """2-norm of the gradients of `params` (an iterable of tensors; those without a gradient are skipped) as an fp32
     0-dim CUDA tensor, summed in 64 bits and in a fixed order.  No host synchronisation."""
@@ -31,8 +35,8 @@ class AdamW(torch.optim.Optimizer):
     state_bits: 32 keeps `exp_avg` and `exp_avg_sq` in fp32 (also for bf16 parameters), under torch's names, and loads
         the state_dict of a torch.optim.AdamW.  8 keeps the first moment and the ROOT of the second as E4M3 codes
         with one power of two per 256 elements (`exp_avg`, `exp_avg_scale`, `exp_avg_root`, `exp_avg_root_scale`; value =
-        code * scale, elements in memory order, which `layout` keeps), rounded stochastically.  A block that holds an infinity, a NaN or a
-        magnitude of 2^51 or more is NaN as a whole from then on.
+        code * scale, elements in memory order, whose strides `layout` keeps), rounded stochastically.  A block that
+        holds an infinity, a NaN or a magnitude of 2^51 or more is NaN as a whole from then on.
     max_norm: clip the gradients to this norm over ALL parameter groups, as clip_grad_norm_ in front of the step would,
         but inside it: `p.grad` itself is left as it is.  The norm of the last step is in `grad_norm` (0-dim, on the
         device).  step(grad_norm=...) takes a norm found elsewhere instead, e.g. one that counts shards on other ranks.
@@ -75,23 +79,16 @@ class AdamW(torch.optim.Optimizer):
         else:
             flat = {}
             for name in _NAMES[8]:
-                n, dtype = (total // BLOCK, torch.float8_e8m0fnu) if name.endswith("_scale") else (total, torch.float8_e4m3fn)
-                flat[name] = torch.zeros(n, dtype=torch.uint8, device=dev).view(dtype)
+                n = total // BLOCK if name.endswith("_scale") else total
+                flat[name] = torch.zeros(n, dtype=torch.uint8, device=dev).view(_dtype8(name))
         self._flat.append(flat)
-        at = 0
-        for p, b in zip(params, blocks):
-            st = {"step": 0}
-            if self.state_bits == 8:                   # (the codes follow the parameter's memory, which must not be reordered)
-                st["layout"] = torch.empty_strided(p.shape, p.stride(), device="meta")
-            for name, buf in flat.items():
-                if name.endswith("_scale"):
-                    st[name] = buf[at:at + b]
-                elif self.state_bits == 8:
-                    st[name] = buf[at * BLOCK:(at + b) * BLOCK]
-                else:
-                    st[name] = buf.as_strided(p.shape, p.stride(), at * BLOCK)
-            self.state[p] = st
-            at += b
+        parts = {name: buf.split(blocks if name.endswith("_scale") else [b * BLOCK for b in blocks]) for name, buf in flat.items()}
+        for i, p in enumerate(params):
+            if self.state_bits == 32:
+                st = {name: t[i].as_strided(p.shape, p.stride()) for name, t in parts.items()}
+            else:                                      # (the codes follow the parameter's memory, which must not be reordered)
+                st = {**{name: t[i] for name, t in parts.items()}, "layout": tuple(p.stride())}
+            self.state[p] = {"step": 0, **st}
 
     def flat_state(self):
         """The buffers that the moments are views into, in the order they were made: one dict per parameter group, and one
@@ -109,23 +106,30 @@ class AdamW(torch.optim.Optimizer):
         for i, st in saved.items():
             if any(n not in st for n in ("step", *names)):
                 raise ValueError(f"the saved state of parameter {i} is not that of {self.state_bits}-bit moments")
+        pairs = [[(saved[i], p) for i, p in zip(old["params"], new["params"]) if i in saved]
+                 for old, new in zip(groups, self.param_groups)]
+        for st, p in (pair for group in pairs for pair in group):
+            if "layout" in st and tuple(st["layout"]) != tuple(p.stride()):
+                raise ValueError(f"the saved moments are in the order of strides {tuple(st['layout'])}, not {p.stride()}")
+            blocks = -(-p.numel() // BLOCK)
+            for n in names:
+                fits = p.numel() if self.state_bits == 32 else blocks if n.endswith("_scale") else blocks * BLOCK
+                if st[n].numel() != fits or (self.state_bits == 8 and st[n].dtype != _dtype8(n)):
+                    raise ValueError(f"the saved {n} does not fit a parameter of shape {tuple(p.shape)}")
         super().load_state_dict({"state": {}, "param_groups": groups})
         self._flat = []
-        for old, new in zip(groups, self.param_groups):
-            pairs = [(saved[i], p) for i, p in zip(old["params"], new["params"]) if i in saved]
-            self._make_state([p for _, p in pairs])
-            for st, p in pairs:
+        to, source = [], []
+        for group in pairs:
+            self._make_state([p for _, p in group])
+            for st, p in group:
                 mine = self.state[p]
                 mine["step"] = int(st["step"])
-                if "layout" in st and (st["layout"].shape, st["layout"].stride()) != (p.shape, p.stride()):
-                    raise ValueError(f"the saved moments are in the order of strides {st['layout'].stride()}, not {p.stride()}")
                 for n in names:
-                    if st[n].numel() != mine[n].numel() or (self.state_bits == 8 and st[n].dtype != mine[n].dtype):
-                        raise ValueError(f"the saved {n} does not fit a parameter of shape {tuple(p.shape)}")
-                    if self.state_bits == 8:
-                        mine[n].view(torch.uint8).copy_(st[n].view(torch.uint8))
-                    else:
-                        mine[n].copy_(st[n])
+                    eight = self.state_bits == 8
+                    to.append(mine[n].view(torch.uint8) if eight else mine[n])
+                    source.append(st[n].view(torch.uint8) if eight else st[n].view(p.shape) if st[n].shape != p.shape else st[n])
+        if to:
+            torch._foreach_copy_(to, source)
 
     # ---- step ----
     def step(self, closure=None, *, grad_norm=None):

@@ -485,3 +485,28 @@ def test_reordered_parameters_are_noticed(optim):
         else:
             other.load_state_dict(saved)               # element by element
             assert torch.equal(other.state[p]["exp_avg"], opt.state[p]["exp_avg"])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_saved_to_a_file_loads_on_any_device(optim, bits, tmp_path):
+    a = _params([(33, 77), (257,), (5,)])
+    x = optim.AdamW(a, **HYPER, state_bits=bits)
+    x.step()
+    torch.save(x.state_dict(), tmp_path / "state.pt")
+    saved = torch.load(tmp_path / "state.pt", map_location="cpu", weights_only=False)
+    b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    for p, q in zip(a, b):
+        q.grad = p.grad.clone()
+    y = optim.AdamW(b, **HYPER, state_bits=bits)
+    y.load_state_dict(saved)
+    x.step()
+    y.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    # what does not fit is refused before anything is touched
+    c = _params([(33, 78), (257,), (5,)])
+    z = optim.AdamW(c, **HYPER, state_bits=bits)
+    z.step()
+    before = z.state[c[1]]["exp_avg"]
+    with pytest.raises(ValueError):
+        z.load_state_dict(saved)
+    assert z.state[c[1]]["exp_avg"] is before and z.state[c[0]]["step"] == 1

@@ -219,21 +219,24 @@ __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
   return r;
 }
 
-// Eight E4M3 codes under an E8M0 scale -> fp32 (every product is exact).
-__device__ __forceinline__ void decode8(uint2 q, uint32_t scale, Eight& x) {
-  const uint32_t f = scale == 255u ? 0x7fc00000u : scale == 0u ? 0x00400000u : scale << 23;
-  const float2 ff = both(__uint_as_float(f));
+__device__ __forceinline__ float scale_of(uint32_t e8m0) {
+  return __uint_as_float(e8m0 == 255u ? 0x7fc00000u : e8m0 == 0u ? 0x00400000u : e8m0 << 23);
+}
+// Eight E4M3 codes -> fp32.
+__device__ __forceinline__ void decode8(uint2 q, Eight& x) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint16_t two = (uint16_t)((j < 2 ? q.x : q.y) >> (16 * (j & 1)));
     uint32_t h;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
-    x.v[j] = mul2(__half22float2(*reinterpret_cast<const __half2*>(&h)), ff);
+    x.v[j] = __half22float2(*reinterpret_cast<const __half2*>(&h));
   }
 }
 
-// Codes of eight elements under the block's scale, which lane 0 stores; d: words of 16 random bits for each.
-template <bool SIGNED> __device__ __forceinline__ uint2 encode8(Eight x, const uint32_t (&d)[8], uint8_t* scale) {
+// Codes of eight elements under the block's scale, which lane 0 stores.  d: a word for two elements, 16 random bits each; the
+// first takes the low ones, or the high ones when the word has been turned round.
+template <bool SIGNED, bool TURNED> __device__ __forceinline__ uint2 encode8(Eight x, const uint32_t (&d)[4], uint8_t* scale) {
+  constexpr uint32_t kLow = 0x0010u, kHigh = 0x1000u;        // 16 bits times 16 and the others times 0: one dot product
   const float top_f = max3_abs_nan(max3_abs_nan(x[0], x[1], x[2]), x[3], x[4]);
   const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(max3_abs_nan(max3_abs_nan(top_f, x[5], x[6]), x[7], x[7])));
   const uint32_t e = min(max(top >> 23, 27u), 177u);
@@ -249,8 +252,8 @@ template <bool SIGNED> __device__ __forceinline__ uint2 encode8(Eight x, const u
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float2 y = mul2(x.v[j], h);
-    u[2 * j] = __float_as_uint(y.x) + (d[2 * j] << 4);       // (the sign bit stays: the magnitude ends at bit 26)
-    u[2 * j + 1] = __float_as_uint(y.y) + (d[2 * j + 1] << 4);
+    u[2 * j] = __dp2a_lo(d[j], TURNED ? kHigh : kLow, __float_as_uint(y.x));         // (the sign bit stays: the
+    u[2 * j + 1] = __dp2a_lo(d[j], TURNED ? kLow : kHigh, __float_as_uint(y.y));     // magnitude ends at bit 26)
   }
   uint32_t w[4];
 #pragma unroll
@@ -314,14 +317,15 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constan
 }
 
 // Roots of two numbers: the approximate reciprocal root and one Newton step with the exact residual (Markstein 1990), which gives
-// the correctly rounded root but for cases too close to call in 44 bits.  What is below 2^-120 comes out smaller than its
-// root, zero as zero: a root under 2^-60 is nothing beside any eps.
+// the correctly rounded root but for cases too close to call in 44 bits.  The smallest normal number is added for zero's sake,
+// whose root is zero; from 2^-100 on that changes nothing, and a root under 2^-50 is nothing beside any eps.
 __device__ __forceinline__ float2 roots(float2 x) {
   float2 y;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(fmaxf(x.x, 0x1p-120f)));
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(fmaxf(x.y, 0x1p-120f)));
+  const float2 z = __fadd2_rn(x, both(0x1p-126f));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(z.x));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(z.y));
   const float2 r = __fmul2_rn(x, y), minus_half = __fmul2_rn(y, both(-0.5f));
-  return __ffma2_rn(__ffma2_rn(r, r, make_float2(-x.x, -x.y)), minus_half, r);
+  return __ffma2_rn(__ffma2_rn(r, r, __fmul2_rn(x, both(-1.0f))), minus_half, r);
 }
 __device__ __forceinline__ float reciprocal_approx(float x) {
   float r;
@@ -331,14 +335,16 @@ __device__ __forceinline__ float reciprocal_approx(float x) {
 
 // The same step on 8-bit moments.  It is bound by instructions as much as by memory (75 for an element with the arithmetic
 // above, 16 or 10 bytes).  The moments keep that arithmetic, so that the codes are those of its definition; in the update the
-// quotient is a product with the approximate reciprocal, and products are fused with their sums: 2^-21 of an update.  49
-// instructions an element are left: 124M fp32 parameters 364 us (5.2 TB/s), 222M bf16 ones 488 (4.5).
+// quotient is a product with the approximate reciprocal, and products are fused with their sums: 2^-21 of an update.  The scale of
+// the first moment goes into beta1, and a dot product of 16-bit halves adds an element's share of a random word.  44 or 45
+// instructions an element are left: 124M fp32 parameters 364 us (5.25 TB/s), 222M bf16 ones 474 (4.7).
 //
 // A warp takes two blocks in a row of fp32 parameters, four of bf16, with the loads of all of them in flight before the
 // first is worked on; the table, the constants and the addresses are worked out once for them.  Two CTAs of 128 registers
 // a thread then beat three or four of fewer (with the moments' arithmetic fused too, 124M fp32 parameters: 355 us, 409 with one
 // block and three CTAs, 411 with one and four; 222M bf16 ones 459, 564, 533), copying ahead to shared memory (353 to 514, 576 to
-// 597) and loading the next run's blocks in the place of each that is done (registers spill: 378 and 532 against 364 and 488).
+// 597) and loading the next run's blocks in the place of each that is done (registers spill: 378 and 532 against 364 and 488).  CTAs
+// of 128 threads make no difference, four on an SM (371 and 466) or five (96 registers, spills: 377 and 536).
 template <class T> constexpr int kRun = 8 / sizeof(T);
 template <class T> constexpr int kChunk8 = kRun<T> * kChunk;
 template <class T> struct Item8 {
@@ -354,12 +360,15 @@ __device__ __forceinline__ void step8(const Item8<T>& x, const Hyper& h, float c
   Eight m, r;
   p = x.param.open();
   const Eight g8 = x.grad.open();
-  decode8(x.first, x.first_scale, m);
-  decode8(x.second, x.second_scale, r);
+  decode8(x.first, m);
+  decode8(x.second, r);
+  const float scale_r = scale_of(x.second_scale);
+  const float2 scaled_beta1 = __fmul2_rn(both(scale_of(x.first_scale)), h.beta1);      // (exact: encode8 makes powers of two of 2^-107 and more)
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float2 g = __fmul2_rn(g8.v[j], both(c));
-    m.v[j] = add2(mul2(m.v[j], h.beta1), mul2(g, h.rest1), h.one);
+    m.v[j] = add2(mul2(m.v[j], scaled_beta1), mul2(g, h.rest1), h.one);
+    r.v[j] = mul2(r.v[j], both(scale_r));
     r.v[j] = roots(add2(mul2(mul2(r.v[j], r.v[j]), h.beta2), mul2(mul2(g, h.rest2), g), h.one));
     const float2 below = __ffma2_rn(r.v[j], h.inv_root, h.eps);
     const float2 ratio = __fmul2_rn(m.v[j], make_float2(reciprocal_approx(below.x), reciprocal_approx(below.y)));
@@ -372,16 +381,9 @@ __device__ __forceinline__ void step8(const Item8<T>& x, const Hyper& h, float c
   }
   const Philox4 y = fused::philox_rounds((uint32_t)group, (uint32_t)(group >> 32), (uint32_t)h.offset,
                                          (uint32_t)(h.offset >> 32), keys);
-  const uint32_t w[4] = {y.x, y.y, y.z, y.w};
-  uint32_t d[8], b[8];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t turned = __brev(w[j]);
-    d[2 * j] = w[j] & 0xffffu; d[2 * j + 1] = w[j] >> 16;
-    b[2 * j] = turned >> 16; b[2 * j + 1] = turned & 0xffffu;
-  }
-  *reinterpret_cast<uint2*>(first) = encode8<true>(m, d, first_scale);
-  *reinterpret_cast<uint2*>(second) = encode8<false>(r, b, second_scale);
+  const uint32_t d[4] = {y.x, y.y, y.z, y.w}, b[4] = {__brev(y.x), __brev(y.y), __brev(y.z), __brev(y.w)};
+  *reinterpret_cast<uint2*>(first) = encode8<true, false>(m, d, first_scale);
+  *reinterpret_cast<uint2*>(second) = encode8<false, true>(r, b, second_scale);
 }
 
 constexpr int kResident8 = 2;

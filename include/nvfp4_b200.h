@@ -380,7 +380,7 @@ int nvfp4_rotary_bf16(const void* q, void* q_out, int q_heads, const void* k, vo
  *   state_bits 32: first = m, second = v, fp32 [n]; the scales are not looked at.
  *   state_bits 8:  first and second hold m and sqrt(v) as E4M3 codes [ceil(n / 256) * 256], first_scale and second_scale one
  *     E8M0 power of two per 256 codes [ceil(n / 256)] (byte 255: the block is NaN, which is what a block with an element
- *     of 2^51 or more, an infinity or a NaN becomes; roots under 2^-60 may come out smaller).  All zero is a valid start.
+ *     of 2^51 or more, an infinity or a NaN becomes; roots under 2^-50 are approximate).  All zero is a valid start.
  *     Codes are rounded stochastically: Philox4x32-10 with key philox_seed and counter (counter_base + element / 8,
  *     philox_offset), 16 bits for each of eight elements in order, low half of a word first; sqrt(v) takes the same 16
  *     bits reversed.

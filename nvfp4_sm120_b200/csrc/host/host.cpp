@@ -481,7 +481,7 @@ void check_state(const at::Tensor& t, c10::Device dev, at::ScalarType type, int6
 }
 
 // One step of every parameter that has a gradient.  groups: the optimizer's param_groups; state: its state.  Returns, with
-// nothing done, "state" when a parameter has no state yet and "capture" when the stream is being captured; None when no
+// nothing done, "capture" when the stream is being captured and else "state" when a parameter has no state yet; None when no
 // parameter has a gradient; else the norm of all gradients (0-dim) if max_norm is given, or True.
 py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c10::optional<double> max_norm, uint64_t seed,
                       const OptTensor& norm_in) {
@@ -505,6 +505,10 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
   static const Name kBetas("betas"), kLr("lr"), kEps("eps"), kDecay("weight_decay"), kParams("params"), kStep("step"),
       kFirst("exp_avg"), kSecond("exp_avg_sq"), kRoot("exp_avg_root"), kFirstScale("exp_avg_scale"),
       kRootScale("exp_avg_root_scale"), kLayout("layout");
+  const auto captured = [&] {
+    const c10::cuda::CUDAGuard guard(*dev);
+    return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
+  };
   const at::NoGradGuard no_grad;
   InOrder states{state.ptr()};
   for (py::handle gh : groups) {
@@ -523,7 +527,7 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
       check_param(p, dev);
       at::Tensor g = grad_like(p, g0);
       PyObject* st = states.find(ph.ptr());
-      if (st == nullptr) return py::str("state");
+      if (st == nullptr) return py::str(captured() ? "capture" : "state");
       if (!PyDict_Check(st)) raise(PyExc_TypeError, "optimizer state holds dicts");
       Item it{};
       it.t.param = p.data_ptr();
@@ -565,8 +569,8 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
     }
   }
   if (items.empty()) return py::none();
+  if (captured()) return py::str("capture");
   const c10::cuda::CUDAGuard guard(*dev);
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return py::str("capture");
   at::Tensor parts, norm;
   const double* parts_p = nullptr;
   const float* norm_p = nullptr;
@@ -755,6 +759,7 @@ struct Preference : torch::autograd::Function<Preference> {
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
     only_once(grads);
+    if (!grads[0].defined()) return tensor_list(6);          // the node behind this one gave no gradient
     return {dlogits(ctx->get_saved_variables(), ctx->saved_data["ignore"].toInt(), {}, grads[0], {}), {}, {}, {}, {}, {}};
   }
 };
@@ -793,6 +798,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
     only_once(grads);
+    if (!grads[0].defined()) return tensor_list(10);
     at::Tensor ready;
     if (auto it = ctx->saved_data.find("grad"); it != ctx->saved_data.end()) {      // (a second backward writes its own)
       ready = it->second.toTensor();

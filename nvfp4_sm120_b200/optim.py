@@ -62,6 +62,13 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.max_norm, self.seed, self.grad_norm, self._flat = state_bits, max_norm, int(seed), None, []
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        params = self.param_groups[-1]["params"]
+        if len(set(params)) != len(params):                # the step takes all of them at the same time
+            self.param_groups.pop()
+            raise ValueError("a parameter stands twice in its group")
+
     def __getstate__(self):
         mine = {k: getattr(self, k) for k in ("state_bits", "max_norm", "seed", "grad_norm", "_flat")}
         return {**super().__getstate__(), **mine}
@@ -101,6 +108,8 @@ class AdamW(torch.optim.Optimizer):
         for g in groups:
             if g.get("amsgrad") or g.get("maximize"):
                 raise ValueError("amsgrad and maximize are not supported")
+            if g["weight_decay"] and not g.get("decoupled_weight_decay", True):
+                raise ValueError("the saved state is that of an optimizer whose weight decay is part of the gradient")
         saved = state_dict["state"]
         names = _NAMES[self.state_bits]
         for i, st in saved.items():

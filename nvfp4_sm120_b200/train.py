@@ -201,7 +201,8 @@ def main():
                 with open(a.out, "a") as f:
                     f.write(line + "\n")
 
-    emit({"event": "start", "backend": a.backend, "optimizer": a.optimizer, "objective": a.objective, "params_non_embedding": tr.model.num_params(), "world": world,
+    emit({"event": "start", "backend": a.backend, "optimizer": a.optimizer, "objective": a.objective,
+          "params_non_embedding": tr.model.num_params(), "world": world,
           "tokens_per_step": a.global_batch * a.seq, "fp4_linears": len(tr.model.fp4_linears()),
           "zipf_entropy_nats": tr.entropy})
     t_start = None

@@ -476,3 +476,24 @@ def test_every_number_of_threads_a_row(losses, rows, vocab, dtype):
     n = int((y != IGNORE).sum())
     off = float(_lse_error(x.detach()).max()) * 1.5 + 4 * U * (float(lp64.abs().max()) + 4)
     _check_grad(torch.autograd.grad(loss, x)[0], x.detach(), y, -1.1 * w / n, off)
+
+
+def test_no_gradient_from_behind_gives_none(losses):
+    class Nothing(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x.clone()
+
+        @staticmethod
+        def backward(ctx, g):
+            return None
+
+    x, y = _logits((2, 3, 17), torch.float32, 1), _labels((2, 3), 17, 1, 0.0)
+    old = torch.zeros(2, 3, device="cuda")
+    for call in (lambda t: losses.token_logprobs(t, y).sum(), lambda t: losses.preference_loss(t, y, old[:, 0])[0],
+                 lambda t: losses.policy_loss(t, y, old, old[:, 0] + 1)[0]):
+        t = x.clone().requires_grad_()
+        Nothing.apply(call(t)).backward()
+        assert t.grad is None or not t.grad.any()
+        call(t).backward()
+        assert t.grad.any()

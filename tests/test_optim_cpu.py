@@ -109,3 +109,28 @@ def test_c_entry_points_check_their_arguments(lib):
     assert pref(Rows(**{**rows, "batch": 3}), 1 << 20) == -2 and pref(r, 16) == -7
     assert L.nvfp4_policy_fwd(c.byref(r), p, p, 3, None, 0.2, 0.2, 0.0, p, p, p, p, p, p, None, 0, 0, p, 16, None) == -7
     assert L.nvfp4_policy_fwd(c.byref(r), p, p, 0, None, 0.2, 0.2, 0.0, p, p, p, p, p, p, None, 0, 0, p, 1 << 20, None) == -2
+
+
+@pytest.mark.filterwarnings("ignore:optimizer contains a parameter group with duplicate parameters")
+def test_a_parameter_stands_once():
+    from nvfp4_sm120_b200.optim import AdamW
+    p, q = torch.nn.Parameter(torch.ones(4)), torch.nn.Parameter(torch.ones(4))
+    with pytest.raises(ValueError, match="twice"):
+        AdamW([p, q, p])
+    opt = AdamW([p])
+    for again in ([q, q], [p], [q, p]):
+        with pytest.raises(ValueError):
+            opt.add_param_group({"params": again})
+    assert [g["params"] for g in opt.param_groups] == [[p]]
+    opt.add_param_group({"params": q, "lr": 0.5})
+    assert len(opt.param_groups) == 2 and opt.param_groups[1]["lr"] == 0.5
+
+
+def test_state_of_coupled_weight_decay_is_refused():
+    from nvfp4_sm120_b200.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(4))
+    p.grad = torch.ones(4)
+    other = torch.optim.Adam([p], weight_decay=0.1)
+    other.step()
+    with pytest.raises(ValueError, match="weight decay"):
+        AdamW([p]).load_state_dict(other.state_dict())

@@ -510,3 +510,28 @@ def test_state_saved_to_a_file_loads_on_any_device(optim, bits, tmp_path):
     with pytest.raises(ValueError):
         z.load_state_dict(saved)
     assert z.state[c[1]]["exp_avg"] is before and z.state[c[0]]["step"] == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_capture_leaves_no_state(optim, bits):
+    """The first step would make the state, in memory that belongs to the graph."""
+    from nvfp4_sm120_b200._lib import NVFP4Error
+    p, q = _params([(64, 3)]), _params([(64, 3)])
+    for a, b in zip(p, q):
+        b.data.copy_(a.data)
+        b.grad.copy_(a.grad)
+    opt, plain = (optim.AdamW(x, max_norm=1.0, state_bits=bits) for x in (p, q))
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph.capture_begin()
+        try:
+            with pytest.raises(NVFP4Error, match="captured"):
+                opt.step()
+        finally:
+            graph.capture_end()
+    torch.cuda.current_stream().wait_stream(side)
+    assert not opt.state and not opt.flat_state()
+    opt.step()
+    plain.step()
+    assert torch.equal(p[0], q[0])

@@ -145,8 +145,9 @@ template <class T> __device__ __forceinline__ void keep(T* p, int64_t at, int64_
 
 // ---- sums of squares -------------------------------------------------------------------------------------------------
 // One double per CTA, summed in a fixed order by whoever reads them.  Squares of fp32 are exact in 64 bits and neither
-// overflow nor underflow there; at the memory's rate the conversions are a third of what the SM can do.  490 MB of fp32: 75 us,
-// 6.5 TB/s; 95 in a training loop, where the L2 is still full of the last step's writes.
+// overflow nor underflow there; at the memory's rate the conversions are a third of what the SM can do.  490 MB of fp32 in
+// a training loop, where the L2 is still full of the last step's writes: 88 us with up to 148 * 16 CTAs, 95 with 148 * 4,
+// 86 with 148 * 24; every CTA of the step adds their sums up again.
 __device__ __forceinline__ double cta_sum(double s) {
   __shared__ double part[kThreads / 32];
 #pragma unroll
@@ -159,7 +160,7 @@ __device__ __forceinline__ double cta_sum(double s) {
   return s;
 }
 
-constexpr int kNormSmall = 64, kNormLarge = 512, kNormGrid = 148 * 4;
+constexpr int kNormSmall = 64, kNormLarge = 512, kNormGrid = 148 * 16;
 template <int CAP> struct NormTable {
   const void* grad[CAP];
   int64_t n[CAP];
@@ -198,7 +199,12 @@ __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__
 
 __device__ __forceinline__ float norm_of(const double* parts, int n) {
   double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += kThreads) s += parts[i];
+  for (int i = threadIdx.x; i < n; i += 5 * kThreads) {      // (half of what one launch leaves is in flight at once)
+    double v[5];
+#pragma unroll
+    for (int u = 0; u < 5; ++u) v[u] = i + u * kThreads < n ? parts[i + u * kThreads] : 0.0;
+    s += (v[0] + v[1]) + (v[2] + v[3]) + v[4];
+  }
   return (float)sqrt(cta_sum(s));
 }
 __global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict__ parts, int n, float* __restrict__ out) {
@@ -276,44 +282,41 @@ __device__ __forceinline__ float clip_factor(const Clip& clip) {
 
 // Both kernels go through the chunks last one first: the norm's pass has just read the gradients in their order, and the last
 // of them are still in L2.
-// 32-bit moments, 124M fp32 parameters: 545 us, 28 bytes each at 6.25 TB/s (a copy: 6.55).
+// 32-bit moments, 124M fp32 parameters: 491 us, 28 bytes each at 7.1 TB/s.  A CTA for each chunk: with four on an SM that go
+// through the chunks in turn some SMs are done early, 545 us; with 8, 16, 64 times as many CTAs 511, 504, 496.
 template <class T, int CAP>
 __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constant__ Table<CAP> t, const Clip clip) {
   const float c = clip_factor(clip);
-  int64_t chunk = (int64_t)t.start[t.count] - 1 - blockIdx.x;
-  if (chunk < 0) return;
-  int k = find(t, (uint32_t)chunk);
-  for (; chunk >= 0; chunk -= gridDim.x) {
-    while (t.start[k] > (uint32_t)chunk) --k;
-    const Entry& e = t.e[k];
-    const Hyper& h = t.h[e.hyper];
-    const int64_t n = e.n, at = (chunk - t.start[k]) * kChunk + threadIdx.x * 8;
-    if (at >= n) continue;
-    const bool whole = e.wide && at + 8 <= n;
-    Raw<T> param, grad;
-    Raw<float> first, second;
-    fetch(static_cast<const T*>(e.param), at, n, whole, param);
-    fetch(static_cast<const T*>(e.grad), at, n, whole, grad);
-    fetch(static_cast<const float*>(e.first), at, n, whole, first);
-    fetch(static_cast<const float*>(e.second), at, n, whole, second);
-    Eight p = param.open(), g = grad.open(), m = first.open(), v = second.open();
+  const uint32_t chunk = t.start[t.count] - 1 - blockIdx.x;
+  const int k = find(t, chunk);
+  const Entry& e = t.e[k];
+  const Hyper& h = t.h[e.hyper];
+  const int64_t n = e.n, at = (int64_t)(chunk - t.start[k]) * kChunk + threadIdx.x * 8;
+  if (at >= n) return;
+  const bool whole = e.wide && at + 8 <= n;
+  Raw<T> param, grad;
+  Raw<float> first, second;
+  fetch(static_cast<const T*>(e.param), at, n, whole, param);
+  fetch(static_cast<const T*>(e.grad), at, n, whole, grad);
+  fetch(static_cast<const float*>(e.first), at, n, whole, first);
+  fetch(static_cast<const float*>(e.second), at, n, whole, second);
+  Eight p = param.open(), g = grad.open(), m = first.open(), v = second.open();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 gg = mul2(g.v[j], both(c));               // (by 1 when nothing is clipped)
-      m.v[j] = add2(mul2(m.v[j], h.beta1), mul2(gg, h.rest1), h.one);
-      v.v[j] = add2(mul2(v.v[j], h.beta2), mul2(mul2(gg, h.rest2), gg), h.one);
-    }
-    keep(static_cast<float*>(e.first), at, n, whole, m);
-    keep(static_cast<float*>(e.second), at, n, whole, v);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 root = make_float2(__fsqrt_rn(v.v[j].x), __fsqrt_rn(v.v[j].y));
-      const float2 below = add2(mul2(root, h.inv_root), h.eps, h.one);
-      const float2 ratio = make_float2(__fdiv_rn(m.v[j].x, below.x), __fdiv_rn(m.v[j].y, below.y));
-      p.v[j] = add2(mul2(p.v[j], h.decay), mul2(ratio, h.step), h.one);
-    }
-    keep(static_cast<T*>(e.param), at, n, whole, p);
+  for (int j = 0; j < 4; ++j) {
+    const float2 gg = mul2(g.v[j], both(c));               // (by 1 when nothing is clipped)
+    m.v[j] = add2(mul2(m.v[j], h.beta1), mul2(gg, h.rest1), h.one);
+    v.v[j] = add2(mul2(v.v[j], h.beta2), mul2(mul2(gg, h.rest2), gg), h.one);
   }
+  keep(static_cast<float*>(e.first), at, n, whole, m);
+  keep(static_cast<float*>(e.second), at, n, whole, v);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 root = make_float2(__fsqrt_rn(v.v[j].x), __fsqrt_rn(v.v[j].y));
+    const float2 below = add2(mul2(root, h.inv_root), h.eps, h.one);
+    const float2 ratio = make_float2(__fdiv_rn(m.v[j].x, below.x), __fdiv_rn(m.v[j].y, below.y));
+    p.v[j] = add2(mul2(p.v[j], h.decay), mul2(ratio, h.step), h.one);
+  }
+  keep(static_cast<T*>(e.param), at, n, whole, p);
 }
 
 // Roots of two numbers: the approximate reciprocal root and one Newton step with the exact residual (Markstein 1990), which gives
@@ -453,7 +456,7 @@ inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintp
 template <class T, bool EIGHT, int CAP>
 int launch_step(const nvfp4_adamw_tensor* ts, int count, const nvfp4_adamw_hyper* hs, int n_hypers, const Clip& clip,
            const PhiloxKeys& keys, cudaStream_t stream) {
-  constexpr int chunk = EIGHT ? kChunk8<T> : kChunk, resident = 148 * (EIGHT ? kResident8 : 4);
+  constexpr int chunk = EIGHT ? kChunk8<T> : kChunk;
   Table<CAP> t;
   uint64_t chunks = 0;
   for (int i = 0; i < count; ++i) {
@@ -474,9 +477,12 @@ int launch_step(const nvfp4_adamw_tensor* ts, int count, const nvfp4_adamw_hyper
     t.h[i] = Hyper{two(s.decay), two(s.beta1), two(s.rest1), two(s.beta2), two(s.rest2), two(-s.step_size),
                    two(s.inv_root_correction), two(s.eps), two(1.0f), s.philox_offset};
   }
-  const unsigned grid = (unsigned)(chunks < resident ? chunks : resident);
-  if constexpr (EIGHT) adamw8_kernel<T, CAP><<<grid, kThreads, 0, stream>>>(t, clip, keys);
-  else adamw_kernel<T, CAP><<<grid, kThreads, 0, stream>>>(t, clip);
+  if constexpr (EIGHT) {
+    constexpr unsigned resident = 148 * kResident8;
+    adamw8_kernel<T, CAP><<<chunks < resident ? (unsigned)chunks : resident, kThreads, 0, stream>>>(t, clip, keys);
+  } else {
+    adamw_kernel<T, CAP><<<(unsigned)chunks, kThreads, 0, stream>>>(t, clip);
+  }
   return cudaGetLastError() == cudaSuccess ? NVFP4_OK : NVFP4_E_LAUNCH;
 }
 

@@ -16,8 +16,9 @@
 // first moment reversed.
 //
 // The tensors come as a table in the kernel's parameters (32 KB of constant memory: nothing to allocate, nothing to copy
-// beforehand, and a captured launch keeps its own).  A CTA takes 2048 elements of one tensor at a time, eight consecutive
-// ones a thread: 32-byte accesses, and one warp is one 256-element block, whose maximum is one redux per moment.
+// beforehand, and a captured launch keeps its own).  A CTA takes one chunk of one tensor, 2048 elements, or with 8-bit moments four or
+// five blocks for each warp, eight consecutive ones a thread: 32-byte accesses, and the maximum of a block
+// is one redux per moment.
 #include <type_traits>
 
 #include <cuda_fp16.h>
@@ -148,16 +149,19 @@ template <class T> __device__ __forceinline__ void keep(T* p, int64_t at, int64_
 // overflow nor underflow there; at the memory's rate the conversions are a third of what the SM can do.  490 MB of fp32 in
 // a training loop, where the L2 is still full of the last step's writes: 88 us with up to 148 * 16 CTAs, 95 with 148 * 4,
 // 86 with 148 * 24; every CTA of the step adds their sums up again.
-__device__ __forceinline__ double cta_sum(double s) {
+template <int R> __device__ __forceinline__ double cta_sum(double (&s)[R]) {
   __shared__ double part[kThreads / 32];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
-  __syncthreads();
-  s = 0.0;
+  for (int r = 0; r < R; ++r) {
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) s += part[w];
-  return s;
+    for (int o = 16; o > 0; o >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
+    if ((threadIdx.x & 31) == 0) part[(threadIdx.x >> 5) + r * (kThreads / R / 32)] = s[r];
+  }
+  __syncthreads();
+  double sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) sum += part[w];
+  return sum;
 }
 
 constexpr int kNormSmall = 64, kNormLarge = 512, kNormGrid = 148 * 16;
@@ -172,7 +176,7 @@ template <int CAP> struct NormTable {
 constexpr int kNormChunk = 4 * kChunk;             // four loads of eight elements in flight in each thread
 template <class T, int CAP>
 __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ NormTable<CAP> t, double* __restrict__ parts) {
-  double sum = 0.0;
+  double sum[1] = {0.0};
   const uint32_t total = t.start[t.count];
   uint32_t c = blockIdx.x;
   int k = c < total ? find(t, c) : 0;
@@ -190,25 +194,28 @@ __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__
       if (at + u * kChunk < n) {
         Eight v = x[u].open();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum = fma((double)v[j], (double)v[j], sum);
+        for (int j = 0; j < 8; ++j) sum[0] = fma((double)v[j], (double)v[j], sum[0]);
       }
   }
-  sum = cta_sum(sum);
-  if (threadIdx.x == 0) parts[blockIdx.x] = sum;
+  const double all = cta_sum<1>(sum);
+  if (threadIdx.x == 0) parts[blockIdx.x] = all;
 }
 
-__device__ __forceinline__ float norm_of(const double* parts, int n) {
-  double s = 0.0;
+// In the order of kThreads threads, however many there are: the norm has the same bits wherever it is found.
+template <int THREADS> __device__ __forceinline__ float norm_of(const double* parts, int n) {
+  constexpr int R = kThreads / THREADS;
+  double s[R] = {};
   for (int i = threadIdx.x; i < n; i += 5 * kThreads) {      // (half of what one launch leaves is in flight at once)
-    double v[5];
+    double v[5 * R];
 #pragma unroll
-    for (int u = 0; u < 5; ++u) v[u] = i + u * kThreads < n ? parts[i + u * kThreads] : 0.0;
-    s += (v[0] + v[1]) + (v[2] + v[3]) + v[4];
+    for (int u = 0; u < 5 * R; ++u) v[u] = i + u * THREADS < n ? parts[i + u * THREADS] : 0.0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r] += (v[r] + v[R + r]) + (v[2 * R + r] + v[3 * R + r]) + v[4 * R + r];
   }
-  return (float)sqrt(cta_sum(s));
+  return (float)sqrt(cta_sum<R>(s));
 }
 __global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict__ parts, int n, float* __restrict__ out) {
-  const float v = norm_of(parts, n);
+  const float v = norm_of<kThreads>(parts, n);
   if (threadIdx.x == 0) *out = v;
 }
 
@@ -271,11 +278,17 @@ template <bool SIGNED, bool TURNED> __device__ __forceinline__ uint2 encode8(Eig
   return make_uint2(__byte_perm(w[0], w[1], 0x6420), __byte_perm(w[2], w[3], 0x6420));
 }
 
-// c = min(1, max_norm / (norm + 1e-6)), 1 without clipping; the first CTA leaves the norm for the caller.
-__device__ __forceinline__ float clip_factor(const Clip& clip) {
-  if (clip.parts == nullptr && clip.norm == nullptr) return 1.0f;
-  const float norm = clip.parts != nullptr ? norm_of(clip.parts, clip.n_parts) : *clip.norm;
+// The norm to clip by, 0 without clipping; the first CTA leaves it for the caller.  Loads of the step may stand between this and
+// its use: then they do not wait for it.
+template <int THREADS> __device__ __forceinline__ float norm_to_clip(const Clip& clip) {
+  if (clip.parts == nullptr && clip.norm == nullptr) return 0.0f;
+  const float norm = clip.parts != nullptr ? norm_of<THREADS>(clip.parts, clip.n_parts) : *clip.norm;
   if (blockIdx.x == 0 && threadIdx.x == 0 && clip.norm_out != nullptr) *clip.norm_out = norm;
+  return norm;
+}
+// c = min(1, max_norm / (norm + 1e-6)), 1 without clipping
+__device__ __forceinline__ float clip_factor(const Clip& clip, float norm) {
+  if (clip.parts == nullptr && clip.norm == nullptr) return 1.0f;
   const float c = __fdiv_rn(clip.max_norm, __fadd_rn(norm, 1e-6f));
   return c > 1.0f ? 1.0f : c;                    // (a NaN stays one)
 }
@@ -286,7 +299,7 @@ __device__ __forceinline__ float clip_factor(const Clip& clip) {
 // through the chunks in turn some SMs are done early, 545 us; with 8, 16, 64 times as many CTAs 511, 504, 496.
 template <class T, int CAP>
 __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constant__ Table<CAP> t, const Clip clip) {
-  const float c = clip_factor(clip);
+  const float norm = norm_to_clip<kThreads>(clip);
   const uint32_t chunk = t.start[t.count] - 1 - blockIdx.x;
   const int k = find(t, chunk);
   const Entry& e = t.e[k];
@@ -300,10 +313,11 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constan
   fetch(static_cast<const T*>(e.grad), at, n, whole, grad);
   fetch(static_cast<const float*>(e.first), at, n, whole, first);
   fetch(static_cast<const float*>(e.second), at, n, whole, second);
+  const float c = clip_factor(clip, norm);
   Eight p = param.open(), g = grad.open(), m = first.open(), v = second.open();
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float2 gg = mul2(g.v[j], both(c));               // (by 1 when nothing is clipped)
+    const float2 gg = mul2(g.v[j], both(c));                 // (by 1 when nothing is clipped)
     m.v[j] = add2(mul2(m.v[j], h.beta1), mul2(gg, h.rest1), h.one);
     v.v[j] = add2(mul2(v.v[j], h.beta2), mul2(mul2(gg, h.rest2), gg), h.one);
   }
@@ -338,18 +352,19 @@ __device__ __forceinline__ float reciprocal_approx(float x) {
 
 // The same step on 8-bit moments.  It is bound by instructions as much as by memory (75 for an element with the arithmetic
 // above, 16 or 10 bytes).  The moments keep that arithmetic, so that the codes are those of its definition; in the update the
-// quotient is a product with the approximate reciprocal, and products are fused with their sums: 2^-21 of an update.  The scale of
-// the first moment goes into beta1, and a dot product of 16-bit halves adds an element's share of a random word.  44 or 45
-// instructions an element are left: 124M fp32 parameters 364 us (5.25 TB/s), 222M bf16 ones 474 (4.7).
+// quotient is a product with the approximate reciprocal, and products are fused with their sums: 2^-21 of an update.  The scale
+// of the first moment goes into beta1, and a dot product of 16-bit halves adds an element's share of a random word.
+// 124M fp32 parameters 281 us (7.0 TB/s), 222M bf16 ones 421 (5.3).
 //
-// A warp takes two blocks in a row of fp32 parameters, four of bf16, with the loads of all of them in flight before the
-// first is worked on; the table, the constants and the addresses are worked out once for them.  Two CTAs of 128 registers
-// a thread then beat three or four of fewer (with the moments' arithmetic fused too, 124M fp32 parameters: 355 us, 409 with one
-// block and three CTAs, 411 with one and four; 222M bf16 ones 459, 564, 533), copying ahead to shared memory (353 to 514, 576 to
-// 597) and loading the next run's blocks in the place of each that is done (registers spill: 378 and 532 against 364 and 488).  CTAs
-// of 128 threads make no difference, four on an SM (371 and 466) or five (96 registers, spills: 377 and 536).
-template <class T> constexpr int kRun = 8 / sizeof(T);
-template <class T> constexpr int kChunk8 = kRun<T> * kChunk;
+// A warp takes four blocks in a row of fp32 parameters, five of bf16, as many as fit in 128 registers, with the loads of all
+// of them in flight before the first is worked on; the table, the constants and the addresses are worked out once for them.  A
+// CTA takes one such chunk and goes, so that its registers go to the loads of the next one while its neighbours compute: eight
+// CTAs of two warps on an SM.  (CTAs that stay and go from chunk to chunk: 364 and 474.  CTAs of 128 threads 285 and 441, of 32
+// 280 and 431; two fp32 blocks 348, three 304, five 308 with spills; four bf16 blocks 432, six 435 with spills; nine CTAs of 96
+// registers 337 and 427, six of 160 294 and 459.)
+template <class T> constexpr int kRun = sizeof(T) == 4 ? 4 : 5;
+constexpr int kThreads8 = 64;
+template <class T> constexpr int kChunk8 = kRun<T> * kThreads8 * 8;
 template <class T> struct Item8 {
   Raw<T> param, grad;
   uint2 first, second;
@@ -389,66 +404,67 @@ __device__ __forceinline__ void step8(const Item8<T>& x, const Hyper& h, float c
   *reinterpret_cast<uint2*>(second) = encode8<false, true>(r, b, second_scale);
 }
 
-constexpr int kResident8 = 2;
 template <class T, int CAP>
-__global__ void __launch_bounds__(kThreads, kResident8) adamw8_kernel(const __grid_constant__ Table<CAP> t, const Clip clip,
-                                                                      const PhiloxKeys keys) {
-  const float c = clip_factor(clip);
-  int64_t chunk = (int64_t)t.start[t.count] - 1 - blockIdx.x;
-  if (chunk < 0) return;
-  int k = find(t, (uint32_t)chunk);
-  for (; chunk >= 0; chunk -= gridDim.x) {
-    while (t.start[k] > (uint32_t)chunk) --k;
-    const Entry& e = t.e[k];
-    const Hyper& h = t.h[e.hyper];
-    const int64_t n = e.n, run = (chunk - t.start[k]) * kChunk8<T> + (threadIdx.x >> 5) * (kRun<T> * kBlock);
-    const int64_t at = run + (threadIdx.x & 31) * 8;
-    if (run >= n) continue;
-    T* param = static_cast<T*>(e.param) + at;
-    const T* grad = static_cast<const T*>(e.grad) + at;
-    uint8_t *first = static_cast<uint8_t*>(e.first) + at, *second = static_cast<uint8_t*>(e.second) + at;
-    uint8_t *first_scale = e.first_scale + run / kBlock, *second_scale = e.second_scale + run / kBlock;
-    const uint64_t group = e.group + (uint64_t)at / 8;
-    Eight p;
-    if (e.wide && run + kRun<T> * kBlock <= n) {
-      Item8<T> x[kRun<T>];
+__global__ void __launch_bounds__(kThreads8, 8) adamw8_kernel(const __grid_constant__ Table<CAP> t, const Clip clip,
+                                                               const PhiloxKeys keys) {
+  const float norm = norm_to_clip<kThreads8>(clip);
+  const uint32_t chunk = t.start[t.count] - 1 - blockIdx.x;
+  const int k = find(t, chunk);
+  const Entry& e = t.e[k];
+  const Hyper& h = t.h[e.hyper];
+  const int64_t n = e.n, run = (int64_t)(chunk - t.start[k]) * kChunk8<T> + (threadIdx.x >> 5) * (kRun<T> * kBlock);
+  const int64_t at = run + (threadIdx.x & 31) * 8;
+  if (run >= n) return;
+  T* param = static_cast<T*>(e.param) + at;
+  const T* grad = static_cast<const T*>(e.grad) + at;
+  uint8_t *first = static_cast<uint8_t*>(e.first) + at, *second = static_cast<uint8_t*>(e.second) + at;
+  uint8_t *first_scale = e.first_scale + run / kBlock, *second_scale = e.second_scale + run / kBlock;
+  const uint64_t group = e.group + (uint64_t)at / 8;
+  Eight p;
+  if (e.wide && run + kRun<T> * kBlock <= n) {
+    Item8<T> x[kRun<T>];
 #pragma unroll
-      for (int u = 0; u < kRun<T>; ++u) {
-        x[u].first = *reinterpret_cast<const uint2*>(first + u * kBlock);
-        x[u].second = *reinterpret_cast<const uint2*>(second + u * kBlock);
-        x[u].first_scale = first_scale[u];
-        x[u].second_scale = second_scale[u];
-        x[u].param.load(param + u * kBlock);
-        x[u].grad.load(grad + u * kBlock);
-      }
+    for (int u = 0; u < kRun<T>; ++u) {
+      x[u].first = *reinterpret_cast<const uint2*>(first + u * kBlock);
+      x[u].second = *reinterpret_cast<const uint2*>(second + u * kBlock);
+      x[u].first_scale = first_scale[u];
+      x[u].second_scale = second_scale[u];
+      x[u].param.load(param + u * kBlock);
+      x[u].grad.load(grad + u * kBlock);
+    }
+    const float c = clip_factor(clip, norm);
 #pragma unroll
-      for (int u = 0; u < kRun<T>; ++u) {
-        step8<T>(x[u], h, c, keys, group + u * (kBlock / 8), 8, p, first + u * kBlock, second + u * kBlock, first_scale + u,
-                 second_scale + u);
-        store8(param + u * kBlock, p);
-      }
-    } else {                                                 // a run that ends in it, or one that lies off the vectors' boundaries
+    for (int u = 0; u < kRun<T>; ++u) {
+      step8<T>(x[u], h, c, keys, group + u * (kBlock / 8), 8, p, first + u * kBlock, second + u * kBlock, first_scale + u,
+               second_scale + u);
+      store8(param + u * kBlock, p);
+    }
+  } else {                                                   // a run that ends in it, or one that lies off the vectors' boundaries
+    const float c = clip_factor(clip, norm);
 #pragma unroll 1
-      for (int u = 0; u < kRun<T> && run + u * kBlock < n; ++u) {
-        const int64_t left = n - at - u * kBlock;            // lanes behind the end but inside the block carry zeros
-        const bool whole = e.wide && left >= 8;
-        Item8<T> x;
-        fetch(param + u * kBlock, 0, left, whole, x.param);
-        fetch(grad + u * kBlock, 0, left, whole, x.grad);
-        x.first = *reinterpret_cast<const uint2*>(first + u * kBlock);
-        x.second = *reinterpret_cast<const uint2*>(second + u * kBlock);
-        x.first_scale = first_scale[u];
-        x.second_scale = second_scale[u];
-        step8<T>(x, h, c, keys, group + u * (kBlock / 8), left, p, first + u * kBlock, second + u * kBlock, first_scale + u,
-                 second_scale + u);
-        keep(param + u * kBlock, 0, left, whole, p);
-      }
+    for (int u = 0; u < kRun<T> && run + u * kBlock < n; ++u) {
+      const int64_t left = n - at - u * kBlock;              // lanes behind the end but inside the block carry zeros
+      const bool whole = e.wide && left >= 8;
+      Item8<T> x;
+      fetch(param + u * kBlock, 0, left, whole, x.param);
+      fetch(grad + u * kBlock, 0, left, whole, x.grad);
+      x.first = *reinterpret_cast<const uint2*>(first + u * kBlock);
+      x.second = *reinterpret_cast<const uint2*>(second + u * kBlock);
+      x.first_scale = first_scale[u];
+      x.second_scale = second_scale[u];
+      step8<T>(x, h, c, keys, group + u * (kBlock / 8), left, p, first + u * kBlock, second + u * kBlock, first_scale + u,
+               second_scale + u);
+      keep(param + u * kBlock, 0, left, whole, p);
     }
   }
 }
 
 template <int CAP> constexpr bool fits() { return sizeof(Table<CAP>) + sizeof(Clip) + sizeof(PhiloxKeys) <= 32764; }
 constexpr int kSmall = 64, kLarge = 400;
+// Parameters from which the norm is found in front of the step on 8-bit moments, by one launch for all its many CTAs (16M 59 us
+// instead of 60, 124M 3 + 281 instead of 318; below, the launch costs more than it saves: 8M 33 instead of 32, 4M 23, not 21).
+// The step on 32-bit moments has twice the warps on an SM to hide the sum behind (124M 495 us, 493 with it in front).
+constexpr double kNormFirst = 12e6;
 static_assert(fits<kLarge>() && sizeof(NormTable<kNormLarge>) + 8 <= 32764, "kernel parameters are 32764 bytes at most");
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
@@ -477,12 +493,8 @@ int launch_step(const nvfp4_adamw_tensor* ts, int count, const nvfp4_adamw_hyper
     t.h[i] = Hyper{two(s.decay), two(s.beta1), two(s.rest1), two(s.beta2), two(s.rest2), two(-s.step_size),
                    two(s.inv_root_correction), two(s.eps), two(1.0f), s.philox_offset};
   }
-  if constexpr (EIGHT) {
-    constexpr unsigned resident = 148 * kResident8;
-    adamw8_kernel<T, CAP><<<chunks < resident ? (unsigned)chunks : resident, kThreads, 0, stream>>>(t, clip, keys);
-  } else {
-    adamw_kernel<T, CAP><<<(unsigned)chunks, kThreads, 0, stream>>>(t, clip);
-  }
+  if constexpr (EIGHT) adamw8_kernel<T, CAP><<<(unsigned)chunks, kThreads8, 0, stream>>>(t, clip, keys);
+  else adamw_kernel<T, CAP><<<(unsigned)chunks, kThreads, 0, stream>>>(t, clip);
   return cudaGetLastError() == cudaSuccess ? NVFP4_OK : NVFP4_E_LAUNCH;
 }
 
@@ -565,9 +577,11 @@ extern "C" int nvfp4_adamw(const nvfp4_adamw_tensor* tensors, int count, const n
   if (sumsq_parts != nullptr && (norm != nullptr || n_parts <= 0)) return NVFP4_E_MODE;
   if (!aligned(sumsq_parts, 8) || !aligned(norm, 4) || !aligned(norm_out, 4)) return NVFP4_E_ALIGN;
   const bool eight = state_bits == 8;
+  double elements = 0.0;
   for (int i = 0; i < count; ++i) {
     const nvfp4_adamw_tensor& s = tensors[i];
     if (s.n <= 0) return NVFP4_E_SHAPE;
+    elements += (double)s.n;
     if (!s.param || !s.grad || !s.first || !s.second || (eight && (!s.first_scale || !s.second_scale))) return NVFP4_E_NULL;
     if (s.hyper < 0 || s.hyper >= n_hypers) return NVFP4_E_MODE;
     const uintptr_t a = is_f32 ? 4 : 2;
@@ -580,9 +594,15 @@ extern "C" int nvfp4_adamw(const nvfp4_adamw_tensor* tensors, int count, const n
     keys.k[r][1] = (uint32_t)(philox_seed >> 32) + (uint32_t)r * 0xBB67AE85u;
   }
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (eight && sumsq_parts != nullptr && norm_out != nullptr && elements > kNormFirst) {
+    norm_kernel<<<1, kThreads, 0, stream>>>(sumsq_parts, n_parts, norm_out);
+    if (cudaGetLastError() != cudaSuccess) return NVFP4_E_LAUNCH;
+    norm = norm_out;
+    sumsq_parts = nullptr;
+  }
   for (int i = 0; i < count; i += kLarge) {
     const int m = count - i < kLarge ? count - i : kLarge;
-    const Clip clip{sumsq_parts, norm, n_parts, max_norm, i == 0 ? norm_out : nullptr};
+    const Clip clip{sumsq_parts, norm, n_parts, max_norm, i == 0 && norm_out != norm ? norm_out : nullptr};
     auto go = [&](auto small) -> int {
       constexpr int cap = decltype(small)::value;
       const nvfp4_adamw_tensor* ts = tensors + i;

@@ -16,9 +16,9 @@
 // first moment reversed.
 //
 // The tensors come as a table in the kernel's parameters (32 KB of constant memory: nothing to allocate, nothing to copy
-// beforehand, and a captured launch keeps its own).  A CTA takes one chunk of one tensor, 2048 elements, or with 8-bit moments four or
-// five blocks for each warp, eight consecutive ones a thread: 32-byte accesses, and the maximum of a block
-// is one redux per moment.
+// beforehand, and a captured launch keeps its own).  A CTA takes one chunk of one tensor, 2048 elements, or with 8-bit
+// moments four or five blocks for each warp, eight consecutive ones a thread: 32-byte accesses, and the maximum of a block is
+// one redux per moment.
 #include <type_traits>
 
 #include <cuda_fp16.h>

@@ -621,7 +621,11 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
                             parts_p == nullptr ? 0 : (int)parts.numel(), norm_p, max_norm.value_or(0.0),
                             norm_out ? float_ptr(norm) : nullptr, stream_of(*dev)),
             "nvfp4_adamw");
-      norm_out = false;
+      if (norm_out) {                                        // later launches take the norm that the first one left
+        parts_p = nullptr;
+        norm_p = float_ptr(norm);
+        norm_out = false;
+      }
     }
   }
   for (const Item& it : items) {

@@ -535,3 +535,26 @@ def test_a_refused_capture_leaves_no_state(optim, bits):
     opt.step()
     plain.step()
     assert torch.equal(p[0], q[0])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("large", [1000, 6_500_003])
+def test_the_norm_is_the_same_wherever_it_is_found(optim, bits, large):
+    """Both dtypes and more tensors than a launch takes: every launch clips by the norm of all gradients."""
+    sets = []
+    for _ in range(2):
+        sets.append(_params([(large,), (large + 5, 2)] + [(37,)] * 420) + _params([(large // 7,), (300,)], torch.bfloat16, 1))
+    p, q = sets
+    norm = optim.grad_norm(q)
+    limit = 0.37 * float(norm)
+    ours, given = (optim.AdamW(x, max_norm=limit, state_bits=bits, **HYPER) for x in (p, q))
+    ours.step()
+    given.step(grad_norm=norm)
+    assert torch.equal(ours.grad_norm, norm)
+    # (one rounding of the norm is two of them in its square; the sums are in 64 bits)
+    assert abs(float(norm) ** 2 - sum(float(x.grad.double().square().sum()) for x in q)) <= 3 * 2.0 ** -24 * float(norm) ** 2
+    for a, b in zip(p, q):
+        assert torch.equal(a, b)
+        for name in ours.state[a]:
+            x, y = ours.state[a][name], given.state[b][name]
+            assert x == y if not isinstance(x, torch.Tensor) else torch.equal(x.view(torch.uint8), y.view(torch.uint8))

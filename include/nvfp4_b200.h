@@ -437,19 +437,25 @@ typedef struct {
   const int64_t* labels;      /* [batch * seq] */
   int64_t ignore_index;
 } nvfp4_logit_rows;           /* HOST struct, read before the call returns */
+/* What the probabilities of a row take: p_v = 2^((x_v - max) log2(e) - log2_sum), log2_sum = log2 sum_v exp(x_v - max).
+ * Two numbers, because their sum in fp32 loses the second beside a large maximum. */
+typedef struct {
+  float max, log2_sum;
+} nvfp4_row_stat;
 /* Scratch of the calls that return a loss: device memory, 16-byte aligned, any content; calls that share it must not overlap. */
 #define NVFP4_LOSS_PARTS 1184
 #define NVFP4_LOSS_WORKSPACE (1024 + 4 * 8 * NVFP4_LOSS_PARTS)
 
 /*
- * logp[row] = x[label] - lse, lse[row] = log sum exp of the row (both 0 for an ignored row).
+ * logp[row] = log softmax(x)[label] (0 for an ignored row); stat [batch * seq], 8-byte aligned, is what the backward pass takes
+ * of each row (zeros for an ignored one).
  * Backward: dlogits ([batch, seq, vocab] of the logits' type with strides of its own, rows that do not overlap; fastest where each
- * row lies as its logits do modulo 16 bytes) = w (onehot(label) - exp(x - lse)), w =
+ * row lies as its logits do modulo 16 bytes) = w (onehot(label) - softmax(x)), w =
  * weight[row / rows_per_weight] (* *scale when given).  unless_one != 0: dlogits already holds the result for a scale of 1, and the
  * call leaves it alone when *scale is 1.  The reference uses torch's cross_entropy (nvfp4_train.py:159-185).
  */
-int nvfp4_logprob_fwd(const nvfp4_logit_rows* rows, float* logp, float* lse, void* stream);
-int nvfp4_logprob_bwd(const nvfp4_logit_rows* rows, const float* lse, const float* weight, int64_t rows_per_weight,
+int nvfp4_logprob_fwd(const nvfp4_logit_rows* rows, float* logp, nvfp4_row_stat* stat, void* stream);
+int nvfp4_logprob_bwd(const nvfp4_logit_rows* rows, const nvfp4_row_stat* stat, const float* weight, int64_t rows_per_weight,
                       const float* scale, int unless_one, void* dlogits, int64_t dstride_b, int64_t dstride_t,
                       void* stream);
 
@@ -461,7 +467,7 @@ int nvfp4_logprob_bwd(const nvfp4_logit_rows* rows, const float* lse, const floa
  * weight[i] = dloss / dL_i, for nvfp4_logprob_bwd with rows_per_weight = seq.  No counterpart in the reference.
  */
 int nvfp4_preference_fwd(const nvfp4_logit_rows* rows, const float* ref, double beta, double label_smoothing, double* logp,
-                         float* lse, float* loss, float* rewards, float* weight, void* workspace, size_t workspace_bytes,
+                         nvfp4_row_stat* stat, float* loss, float* rewards, float* weight, void* workspace, size_t workspace_bytes,
                          void* stream);
 
 /*
@@ -473,7 +479,7 @@ int nvfp4_preference_fwd(const nvfp4_logit_rows* rows, const float* ref, double 
  * No counterpart in the reference.
  */
 int nvfp4_policy_fwd(const nvfp4_logit_rows* rows, const float* old_logp, const float* advantage, int64_t rows_per_advantage,
-                     const float* ref_logp, double clip_low, double clip_high, double kl, float* logp, float* lse, float* weight,
+                     const float* ref_logp, double clip_low, double clip_high, double kl, float* logp, nvfp4_row_stat* stat, float* weight,
                      float* terms, float* loss, float* stats2, void* dlogits, int64_t dstride_b, int64_t dstride_t,
                      void* workspace, size_t workspace_bytes, void* stream);
 

@@ -699,7 +699,8 @@ void only_once(const tensor_list& grads) {
   for (const at::Tensor& g : grads)
     if (g.defined() && g.requires_grad()) throw std::runtime_error("the losses on logits are differentiable once");
 }
-// Gradient of the logits.  saved: logits, labels and, in one tensor, the rows' logsumexp and dloss / dlogp (one per row or per
+nvfp4_row_stat* stat_ptr(const at::Tensor& t) { return reinterpret_cast<nvfp4_row_stat*>(float_ptr(t)); }
+// Gradient of the logits.  saved: logits, labels and, in one tensor, the rows' statistics and dloss / dlogp (one per row or per
 // sequence), or the former alone and `weight` for the latter; scale: what dloss / dlogp is to be multiplied with (one
 // element); ready: the gradient for a scale of 1, used again where the scale is 1
 at::Tensor dlogits(const torch::autograd::variable_list& saved, int64_t ignore, const at::Tensor& weight, const at::Tensor& scale,
@@ -709,10 +710,10 @@ at::Tensor dlogits(const torch::autograd::variable_list& saved, int64_t ignore, 
   const int64_t n = in.count();
   const at::Tensor w = weight.defined() ? weight.to(at::kFloat).contiguous() : saved[2],
                    sc = scale.defined() ? scale.to(at::kFloat) : scale;
-  const float* wp = float_ptr(w) + (weight.defined() ? 0 : n);
-  const int64_t per = n / (weight.defined() ? n : saved[2].numel() - n);
+  const float* wp = float_ptr(w) + (weight.defined() ? 0 : 2 * n);
+  const int64_t per = n / (weight.defined() ? n : saved[2].numel() - 2 * n);
   at::Tensor out = ready.defined() ? ready : gradient_like(saved[0], in);
-  check_in_backward(lib.nvfp4_logprob_bwd(&in.rows, float_ptr(saved[2]), wp, per, sc.defined() ? float_ptr(sc) : nullptr,
+  check_in_backward(lib.nvfp4_logprob_bwd(&in.rows, stat_ptr(saved[2]), wp, per, sc.defined() ? float_ptr(sc) : nullptr,
                                           ready.defined(), out.data_ptr(), batch_stride(out), out.stride(-2), stream_of(in.dev)),
                     "nvfp4_logprob_bwd");
   return out;
@@ -722,9 +723,9 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& labels, int64_t ignore) {
     const Logits in(logits, labels, ignore);
     const c10::cuda::CUDAGuard guard(in.dev);
-    at::Tensor logp = in.per_row(), lse = in.per_row();
-    check(lib.nvfp4_logprob_fwd(&in.rows, float_ptr(logp), float_ptr(lse), stream_of(in.dev)), "nvfp4_logprob_fwd");
-    ctx->save_for_backward({logits, labels, lse});
+    at::Tensor logp = in.per_row(), kept = at::empty({2 * in.count()}, on(in.dev, at::kFloat));
+    check(lib.nvfp4_logprob_fwd(&in.rows, float_ptr(logp), stat_ptr(kept), stream_of(in.dev)), "nvfp4_logprob_fwd");
+    ctx->save_for_backward({logits, labels, kept});
     ctx->saved_data["ignore"] = ignore;
     return logp;
   }
@@ -748,11 +749,11 @@ struct Preference : torch::autograd::Function<Preference> {
     const c10::cuda::CUDAGuard guard(in.dev);
     const int64_t n = in.count();
     at::Tensor loss = at::empty({}, on(in.dev, at::kFloat)), rewards = at::empty({in.rows.batch}, on(in.dev, at::kFloat)),
-               kept = at::empty({n + in.rows.batch}, on(in.dev, at::kFloat));
+               kept = at::empty({2 * n + in.rows.batch}, on(in.dev, at::kFloat));
     const at::Tensor scratch = loss_scratch(in.dev, 8 * n);
     uint8_t* ws = scratch.data_ptr<uint8_t>();
     check(lib.nvfp4_preference_fwd(&in.rows, float_ptr(r), beta, smoothing, reinterpret_cast<double*>(ws + NVFP4_LOSS_WORKSPACE),
-                                   float_ptr(kept), float_ptr(loss), float_ptr(rewards), float_ptr(kept) + n, ws, NVFP4_LOSS_WORKSPACE,
+                                   stat_ptr(kept), float_ptr(loss), float_ptr(rewards), float_ptr(kept) + 2 * n, ws, NVFP4_LOSS_WORKSPACE,
                                    stream_of(in.dev)),
           "nvfp4_preference_fwd");
     ctx->save_for_backward({logits, labels, kept});
@@ -782,13 +783,13 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     at::Tensor rf, grad;
     if (ref.has_value()) rf = in.vec(*ref, n, "ref_logps");
     const c10::cuda::CUDAGuard guard(in.dev);
-    at::Tensor logp = in.per_row(), kept = at::empty({2 * n}, on(in.dev, at::kFloat)), loss = at::empty({}, on(in.dev, at::kFloat)),
+    at::Tensor logp = in.per_row(), kept = at::empty({3 * n}, on(in.dev, at::kFloat)), loss = at::empty({}, on(in.dev, at::kFloat)),
                stats = at::empty({2}, on(in.dev, at::kFloat));
     if (want_grad) grad = gradient_like(logits, in);
     const at::Tensor scratch = loss_scratch(in.dev, 8 * n);
     uint8_t* ws = scratch.data_ptr<uint8_t>();
     check(lib.nvfp4_policy_fwd(&in.rows, float_ptr(old), float_ptr(adv), n / adv.numel(), rf.defined() ? float_ptr(rf) : nullptr,
-                               low, high, kl, float_ptr(logp), float_ptr(kept), float_ptr(kept) + n,
+                               low, high, kl, float_ptr(logp), stat_ptr(kept), float_ptr(kept) + 2 * n,
                                reinterpret_cast<float*>(ws + NVFP4_LOSS_WORKSPACE), float_ptr(loss), float_ptr(stats),
                                want_grad ? grad.data_ptr() : nullptr, want_grad ? batch_stride(grad) : 0,
                                want_grad ? grad.stride(-2) : 0, ws, NVFP4_LOSS_WORKSPACE, stream_of(in.dev)),

@@ -1,8 +1,8 @@
 // Losses on logits and their gradients (sm_100a): log-probabilities of given labels, a preference loss over pairs of
 // sequences, a clipped policy loss with a KL term.
 //
-//   lse = M + log sum_v exp(x_v - M)        logp = x[label] - lse (0 where the label is the ignored one)
-//   dx_v = w (onehot_v - exp(x_v - lse))    with w = dloss / dlogp of the row
+//   S = sum_v exp(x_v - M), M the row's maximum     logp = (x[label] - M) - log S (0 where the label is the ignored one)
+//   dx_v = w (onehot_v - exp(x_v - M) / S)          with w = dloss / dlogp of the row
 //   preference: L_i = sum_t logp_it, reward_i = beta (L_i - ref_i), h = reward_chosen - reward_rejected,
 //               loss = mean over pairs of -(1 - s) logsigmoid(h) - s logsigmoid(-h);
 //               w_chosen = beta / P (s sigmoid(h) - (1 - s) sigmoid(-h)) = -w_rejected
@@ -11,7 +11,9 @@
 //
 // A row of logits is read once with a running maximum and sum per thread, the group's are joined at the end: fp32, base
 // 2, the maximum subtracted before the product with log2 e, so that rows of the type's lowest value give no infinity.
-// The maximum starts at the lowest finite number, not at -inf: a row of -inf then ends with a sum of 0 and lse = -inf.
+// The maximum starts at the lowest finite number, not at -inf: a row of -inf then ends with a sum of 0, and is NaN.
+// M and log2 S go from the forward to the backward pass apart: added up, log S would be lost beside a maximum of 1e9 (a row of
+// one mask value) and off by 5e-4 beside one of 1e4, and with it all of the row's gradient.
 // A row belongs to a warp or to a CTA of 128 to 512 threads, by its length and the number of rows (group_of).
 // The policy loss's w depends on its own row alone, so its kernel writes the row's gradient right behind the sum, while
 // the row is in L2: HBM sees each row once.  The preference loss has to see both sequences first; its backward takes the
@@ -43,6 +45,7 @@ struct Rows {
 struct Stat {
   float m, s;
 };
+using Norm = nvfp4_row_stat;                      // what a row's probabilities take: its maximum and the base-2 logarithm of that sum
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -56,10 +59,10 @@ __device__ __forceinline__ float2 exp_of(float2 d) {
   const float2 t = __ffma2_rn(d, both(kLog2e), __fmul2_rn(d, both(kLog2eRest)));
   return make_float2(ex2(t.x), ex2(t.y));
 }
-// the same within 1.3e-8 d of itself: enough for a gradient
-__device__ __forceinline__ float exp_near(float d) { return ex2(d * kLog2e); }
-__device__ __forceinline__ float2 exp_near(float2 d) {
-  const float2 t = __fmul2_rn(d, both(kLog2e));
+// exp(d) / S within 1.3e-8 d of itself: enough for a gradient.  less: -log2 S
+__device__ __forceinline__ float exp_near(float d, float less) { return ex2(fmaf(d, kLog2e, less)); }
+__device__ __forceinline__ float2 exp_near(float2 d, float2 less) {
+  const float2 t = __ffma2_rn(d, both(kLog2e), less);
   return make_float2(ex2(t.x), ex2(t.y));
 }
 // max(m, a, b) as one three-input instruction (a NaN does not count; it shows in the sum)
@@ -68,13 +71,14 @@ __device__ __forceinline__ float max3(float m, float a, float b) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
   return r;
 }
-// M + log s.  The sum's exponent is taken off in front of the logarithm, whose own rounding is then far below that of an fp32
+// log s.  The sum's exponent is taken off in front of the logarithm, whose own rounding is then far below that of an fp32
 // result.  (Beside a coarse maximum, logf(s) would leave every other result halfway between two fp32 numbers.)
-__device__ __forceinline__ double lse_of(Stat st) {
-  const int k = min(max((int)(__float_as_uint(st.s) >> 23) - 127, 0), 63);       // s is 1 to 2^31, or 0, or no number
-  const float f = st.s * __uint_as_float((uint32_t)(127 - k) << 23);
-  return (double)st.m + (k * 0.69314718055994531 + (double)logf(f));
+__device__ __forceinline__ double log_of(float s) {
+  const int k = min(max((int)(__float_as_uint(s) >> 23) - 127, 0), 63);          // s is 1 to 2^31, or 0, or no number
+  const float f = s * __uint_as_float((uint32_t)(127 - k) << 23);
+  return k * 0.69314718055994531 + (double)logf(f);
 }
+__device__ __forceinline__ Norm norm_of(Stat st, double log_s) { return Norm{st.m, (float)(log_s * 1.4426950408889634)}; }
 
 // A 16-byte vector of logits as pairs of fp32, and back.
 template <class T> struct Vec;
@@ -207,37 +211,38 @@ template <class T, int GROUP> __device__ __forceinline__ void clear_row(T* out, 
   for (uint32_t i = tid; i < vecs; i += GROUP) q[i] = make_uint4(0u, 0u, 0u, 0u);
   for (uint32_t j = tail + tid; j < n; j += GROUP) out[j] = from_float<T>(0.0f);
 }
-// out = w (onehot - exp(x - lse)); w = 0 gives zeros unless the row holds something that is no number
+// out = w (onehot - exp(x - M) / S); w = 0 gives zeros unless the row holds something that is no number
 template <class T> struct GradRow {
   static constexpr int V = Vec<T>::n;
-  float lse, w;
+  Norm norm;
+  float w;
   uint32_t label;
-  __device__ __forceinline__ GradRow(float lse_, float w_, uint32_t label_) : lse(lse_), w(w_), label(label_) {}
+  __device__ __forceinline__ GradRow(Norm norm_, float w_, uint32_t label_) : norm(norm_), w(w_), label(label_) {}
   __device__ __forceinline__ void one(const T* x, T* out, uint32_t i) const {
-    const float p = exp_near(as_float(x[i]) - lse);
+    const float p = exp_near(as_float(x[i]) - norm.max, -norm.log2_sum);
     out[i] = from_float<T>(i == label ? __fmaf_rn(-w, p, w) : __fmul_rn(-w, p));
   }
   __device__ __forceinline__ uint4 cold(const uint4& q) const {      // a vector that does not hold the label
-    const float2 below = both(-lse), minus = both(-w);
+    const float2 below = both(-norm.max), less = both(-norm.log2_sum), minus = both(-w);
     float2 v[V / 2];
     Vec<T>::open(q, v);
 #pragma unroll
-    for (int j = 0; j < V / 2; ++j) v[j] = __fmul2_rn(minus, exp_near(__fadd2_rn(v[j], below)));
+    for (int j = 0; j < V / 2; ++j) v[j] = __fmul2_rn(minus, exp_near(__fadd2_rn(v[j], below), less));
     return Vec<T>::close(v);
   }
   __device__ __forceinline__ uint4 hot(const uint4& q, uint32_t at) const {      // one that holds it, as element `at`
-    const float2 below = both(-lse), minus = both(-w);
+    const float2 below = both(-norm.max), less = both(-norm.log2_sum), minus = both(-w);
     float2 v[V / 2];
     Vec<T>::open(q, v);
 #pragma unroll
     for (int j = 0; j < V / 2; ++j)
-      v[j] = __ffma2_rn(minus, exp_near(__fadd2_rn(v[j], below)), make_float2(at == 2 * j ? w : 0.0f, at == 2 * j + 1 ? w : 0.0f));
+      v[j] = __ffma2_rn(minus, exp_near(__fadd2_rn(v[j], below), less), make_float2(at == 2 * j ? w : 0.0f, at == 2 * j + 1 ? w : 0.0f));
     return Vec<T>::close(v);
   }
 };
 template <class T, int GROUP, int UNROLL>
-__device__ __forceinline__ void grad_row(const T* x, T* out, uint32_t n, uint32_t label, float lse, float w, uint32_t tid) {
-  const GradRow<T> g(lse, w, label);
+__device__ __forceinline__ void grad_row(const T* x, T* out, uint32_t n, uint32_t label, Norm norm, float w, uint32_t tid) {
+  const GradRow<T> g(norm, w, label);
   const uint32_t head = lead(x, n), vecs = (n - head) / Vec<T>::n, tail = head + vecs * Vec<T>::n;
   if (lead(out, n) != head) {                     // the two rows lie differently: element by element
     for (uint32_t i = tid; i < n; i += GROUP) g.one(x, out, i);
@@ -286,22 +291,22 @@ template <int GROUP> struct Group {               // a row's threads: a warp of 
 // L: fp32 for the caller, fp64 for the preference loss, whose rewards are small differences of long sums
 template <class T, int GROUP, class L>
 __global__ void __launch_bounds__(Group<GROUP>::threads, 1024 / Group<GROUP>::threads)
-forward_kernel(const Rows r, L* __restrict__ logp, float* __restrict__ lse_out, unsigned int* __restrict__ ticket) {
+forward_kernel(const Rows r, L* __restrict__ logp, Norm* __restrict__ norms, unsigned int* __restrict__ ticket) {
   using G = Group<GROUP>;
   if (ticket != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;      // for the kernel behind this one
   const int64_t row = G::row();
   if (row >= r.rows) return;
   const int64_t label = r.labels[row];
   if (label == r.ignore) {
-    if (G::tid() == 0) { logp[row] = (L)0; lse_out[row] = 0.0f; }
+    if (G::tid() == 0) { logp[row] = (L)0; norms[row] = Norm{0.0f, 0.0f}; }
     return;
   }
   const T* x = row_of<T>(r, row);
   const Stat st = join_group<GROUP>(scan<T, GROUP>(x, r.vocab, G::tid()));
   if (G::tid() == 0) {
-    const double lse = lse_of(st);
-    lse_out[row] = (float)lse;
-    logp[row] = (L)((double)at_label(x, label, r.vocab) - lse);
+    const double log_s = log_of(st.s);
+    norms[row] = norm_of(st, log_s);
+    logp[row] = (L)(((double)at_label(x, label, r.vocab) - (double)st.m) - log_s);
   }
 }
 
@@ -309,7 +314,7 @@ forward_kernel(const Rows r, L* __restrict__ logp, float* __restrict__ lse_out, 
 // w of row i: weight[i / per] (* *scale).  UNLESS_ONE: nothing is left to do when *scale is 1, which is most often so: then few
 // CTAs are launched, which go through the rows in turn where they have to.
 template <class T, int GROUP, bool UNLESS_ONE>
-__global__ void __launch_bounds__(Group<GROUP>::threads) backward_kernel(const Rows r, const float* __restrict__ lse,
+__global__ void __launch_bounds__(Group<GROUP>::threads) backward_kernel(const Rows r, const Norm* __restrict__ norms,
                                                                          const float* __restrict__ weight, uint32_t per,
                                                                          const float* __restrict__ scale, const Out<T> out) {
   using G = Group<GROUP>;
@@ -318,13 +323,13 @@ __global__ void __launch_bounds__(Group<GROUP>::threads) backward_kernel(const R
     const int64_t row = r.rows - 1 - i, label = r.labels[row];
     T* o = out.row(row, r.seq);
     float w = label == r.ignore ? 0.0f : weight[row / per] * by;
-    const float l = lse[row];
-    if (label == r.ignore || (w == 0.0f && fabsf(l) <= FLT_MAX)) {
+    const Norm norm = norms[row];
+    if (label == r.ignore || (w == 0.0f && fabsf(norm.max) <= FLT_MAX && fabsf(norm.log2_sum) <= FLT_MAX)) {
       clear_row<T, GROUP>(o, r.vocab, G::tid());
       return;
     }
     if (label < 0 || label >= (int64_t)r.vocab) w = __uint_as_float(0x7fc00000u);
-    grad_row<T, GROUP, 2>(row_of<T>(r, row), o, r.vocab, (uint32_t)label, l, w, G::tid());
+    grad_row<T, GROUP, 2>(row_of<T>(r, row), o, r.vocab, (uint32_t)label, norm, w, G::tid());
   };
   if constexpr (UNLESS_ONE) {
     if (by == 1.0f) return;
@@ -451,7 +456,7 @@ __device__ __forceinline__ float share_of(unsigned int counts) {
 
 struct PolicyOut {
   float* logp;              // [rows]
-  float* lse;               // [rows]
+  Norm* norm;               // [rows]
   float* weight;            // [rows]: dloss / dlogp
   float* term;              // [2, rows]: the row's loss; its KL term, with the sign set where the clamp cut the gradient
 };
@@ -463,9 +468,9 @@ template <class T> __device__ __forceinline__ RowIn row_in(const Policy& p, int6
   return RowIn{p.advantage[row / p.per], p.old[row], p.ref != nullptr ? p.ref[row] : 0.0f, at_label(x, label, vocab)};
 }
 // The row's results, stored by its first thread, and its weight.
-__device__ __forceinline__ float policy_row(const Policy& p, const PolicyOut& o, int64_t rows, int64_t row, const RowIn& in, double lse64,
-                                            float share, bool store) {
-  const float logp = (float)((double)in.x - lse64), a = in.advantage, rho = expf(logp - in.old);
+__device__ __forceinline__ float policy_row(const Policy& p, const PolicyOut& o, int64_t rows, int64_t row, const RowIn& in, float logp,
+                                            Norm norm, float share, bool store) {
+  const float a = in.advantage, rho = expf(logp - in.old);
   const float s = rho * a, q = fminf(fmaxf(rho, p.low), p.high) * a;
   const bool clipped = s > q;                                // (not when it is no number: that has to show)
   float w = clipped ? 0.0f : -s, kl = 0.0f;
@@ -477,7 +482,7 @@ __device__ __forceinline__ float policy_row(const Policy& p, const PolicyOut& o,
   w *= share;
   if (store) {
     o.logp[row] = logp;
-    o.lse[row] = (float)lse64;
+    o.norm[row] = norm;
     o.weight[row] = w;
     o.term[row] = fmaf(p.kl, kl, -(clipped ? q : s));
     o.term[rows + row] = clipped ? -kl : kl;
@@ -485,7 +490,8 @@ __device__ __forceinline__ float policy_row(const Policy& p, const PolicyOut& o,
   return w;
 }
 __device__ __forceinline__ void no_row(const PolicyOut& o, int64_t rows, int64_t row) {
-  o.logp[row] = o.lse[row] = o.weight[row] = o.term[row] = o.term[rows + row] = 0.0f;
+  o.logp[row] = o.weight[row] = o.term[row] = o.term[rows + row] = 0.0f;
+  o.norm[row] = Norm{0.0f, 0.0f};
 }
 
 // One group for each row, which it reads twice when it writes the gradient: the second time from L2.
@@ -505,9 +511,11 @@ __global__ void __launch_bounds__(Group<GROUP>::threads) policy_kernel(const Row
   const T* x = row_of<T>(r, row);
   const RowIn in = row_in(p, row, x, label, r.vocab);
   const Stat st = join_group<GROUP>(scan<T, GROUP>(x, r.vocab, G::tid()));
-  const double lse = lse_of(st);
-  const float w = policy_row(p, o, r.rows, row, in, lse, share_of(counts), G::tid() == 0);
-  if (grad.x != nullptr) grad_row<T, GROUP, 8>(x, grad.row(row, r.seq), r.vocab, (uint32_t)label, (float)lse, w, G::tid());
+  const double log_s = log_of(st.s);
+  const Norm norm = norm_of(st, log_s);
+  const float logp = (float)(((double)in.x - (double)st.m) - log_s);
+  const float w = policy_row(p, o, r.rows, row, in, logp, norm, share_of(counts), G::tid() == 0);
+  if (grad.x != nullptr) grad_row<T, GROUP, 8>(x, grad.row(row, r.seq), r.vocab, (uint32_t)label, norm, w, G::tid());
 }
 
 // Means over the rows with a label, in 64 bits and in a fixed order.
@@ -576,10 +584,10 @@ template <class F> void by_rows(bool f32, const Rows& r, bool writes, F f) {
   else sized(__nv_bfloat16());
 }
 // (16384 rows of 50257 bf16: 246 us, 6.7 TB/s, with eight CTAs of 128 threads an SM; 262 with four of 256)
-template <class L> void forward(const Rows& r, bool f32, L* logp, float* lse, unsigned int* ticket, cudaStream_t stream) {
+template <class L> void forward(const Rows& r, bool f32, L* logp, Norm* norms, unsigned int* ticket, cudaStream_t stream) {
   by_rows(f32, r, false, [&](auto t, auto g, unsigned grid) {
     constexpr int G = decltype(g)::value;
-    forward_kernel<decltype(t), G, L><<<grid, Group<G>::threads, 0, stream>>>(r, logp, lse, ticket);
+    forward_kernel<decltype(t), G, L><<<grid, Group<G>::threads, 0, stream>>>(r, logp, norms, ticket);
   });
 }
 
@@ -603,50 +611,50 @@ void policy_rows(const Rows& r, bool f32, const Policy& p, Words* words, int cou
 
 using namespace nvfp4::logprob;
 
-extern "C" int nvfp4_logprob_fwd(const nvfp4_logit_rows* in, float* logp, float* lse, void* stream_) {
+extern "C" int nvfp4_logprob_fwd(const nvfp4_logit_rows* in, float* logp, nvfp4_row_stat* stat, void* stream_) {
   Rows r;
   if (const int code = check_rows(in, r); code != NVFP4_OK) return code;
-  if (!logp || !lse) return NVFP4_E_NULL;
-  if (!aligned(logp, 4) || !aligned(lse, 4)) return NVFP4_E_ALIGN;
-  forward(r, in->is_f32 != 0, logp, lse, nullptr, static_cast<cudaStream_t>(stream_));
+  if (!logp || !stat) return NVFP4_E_NULL;
+  if (!aligned(logp, 4) || !aligned(stat, 8)) return NVFP4_E_ALIGN;
+  forward(r, in->is_f32 != 0, logp, stat, nullptr, static_cast<cudaStream_t>(stream_));
   return launched();
 }
 
-extern "C" int nvfp4_logprob_bwd(const nvfp4_logit_rows* in, const float* lse, const float* weight, int64_t rows_per_weight,
+extern "C" int nvfp4_logprob_bwd(const nvfp4_logit_rows* in, const nvfp4_row_stat* stat, const float* weight, int64_t rows_per_weight,
                                  const float* scale, int unless_one, void* dlogits, int64_t dstride_b, int64_t dstride_t,
                                  void* stream_) {
   Rows r;
   if (const int code = check_rows(in, r); code != NVFP4_OK) return code;
-  if (!lse || !weight || !dlogits || (unless_one && !scale)) return NVFP4_E_NULL;
+  if (!stat || !weight || !dlogits || (unless_one && !scale)) return NVFP4_E_NULL;
   if (rows_per_weight <= 0 || rows_per_weight > 0x7fffffffLL) return NVFP4_E_SHAPE;
-  if (!aligned(lse, 4) || !aligned(weight, 4) || !aligned(scale, 4) || !aligned(dlogits, in->is_f32 ? 4 : 2)) return NVFP4_E_ALIGN;
+  if (!aligned(stat, 8) || !aligned(weight, 4) || !aligned(scale, 4) || !aligned(dlogits, in->is_f32 ? 4 : 2)) return NVFP4_E_ALIGN;
   by_rows(in->is_f32 != 0, r, true, [&](auto t, auto g, unsigned grid) {
     using T = decltype(t);
     constexpr int G = decltype(g)::value;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const Out<T> out{static_cast<T*>(dlogits), dstride_b, dstride_t};
     const uint32_t per = (uint32_t)rows_per_weight;
-    if (unless_one) backward_kernel<T, G, true><<<grid < 148 * 4 ? grid : 148 * 4, Group<G>::threads, 0, stream>>>(r, lse, weight, per, scale, out);
-    else backward_kernel<T, G, false><<<grid, Group<G>::threads, 0, stream>>>(r, lse, weight, per, scale, out);
+    if (unless_one) backward_kernel<T, G, true><<<grid < 148 * 4 ? grid : 148 * 4, Group<G>::threads, 0, stream>>>(r, stat, weight, per, scale, out);
+    else backward_kernel<T, G, false><<<grid, Group<G>::threads, 0, stream>>>(r, stat, weight, per, scale, out);
   });
   return launched();
 }
 
 extern "C" int nvfp4_preference_fwd(const nvfp4_logit_rows* in, const float* ref, double beta, double label_smoothing, double* logp,
-                                    float* lse, float* loss, float* rewards, float* weight, void* workspace,
+                                    nvfp4_row_stat* stat, float* loss, float* rewards, float* weight, void* workspace,
                                     size_t workspace_bytes, void* stream_) {
   Rows r;
   if (const int code = check_rows(in, r); code != NVFP4_OK) return code;
   if (in->batch % 2 != 0) return NVFP4_E_SHAPE;
-  if (!ref || !logp || !lse || !loss || !rewards || !weight || !workspace) return NVFP4_E_NULL;
+  if (!ref || !logp || !stat || !loss || !rewards || !weight || !workspace) return NVFP4_E_NULL;
   if (workspace_bytes < NVFP4_LOSS_WORKSPACE) return NVFP4_E_WORKSPACE;
-  if (!aligned(ref, 4) || !aligned(logp, 8) || !aligned(lse, 4) || !aligned(loss, 4) || !aligned(rewards, 4) || !aligned(weight, 4) ||
+  if (!aligned(ref, 4) || !aligned(logp, 8) || !aligned(stat, 8) || !aligned(loss, 4) || !aligned(rewards, 4) || !aligned(weight, 4) ||
       !aligned(workspace, 16))
     return NVFP4_E_ALIGN;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   unsigned int* ticket = static_cast<unsigned int*>(workspace);
   double* parts = reinterpret_cast<double*>(static_cast<char*>(workspace) + 16);
-  forward(r, in->is_f32 != 0, logp, lse, ticket, stream);
+  forward(r, in->is_f32 != 0, logp, stat, ticket, stream);
   if (const int code = launched(); code != NVFP4_OK) return code;
   const int64_t pairs = in->batch / 2;
   preference_kernel<<<(unsigned)(pairs < NVFP4_LOSS_PARTS ? pairs : NVFP4_LOSS_PARTS), kThreads, 0, stream>>>(
@@ -656,14 +664,14 @@ extern "C" int nvfp4_preference_fwd(const nvfp4_logit_rows* in, const float* ref
 
 extern "C" int nvfp4_policy_fwd(const nvfp4_logit_rows* in, const float* old_logp, const float* advantage,
                                 int64_t rows_per_advantage, const float* ref_logp, double clip_low, double clip_high, double kl,
-                                float* logp, float* lse, float* weight, float* terms, float* loss, float* stats2, void* dlogits,
+                                float* logp, nvfp4_row_stat* stat, float* weight, float* terms, float* loss, float* stats2, void* dlogits,
                                 int64_t dstride_b, int64_t dstride_t, void* workspace, size_t workspace_bytes, void* stream_) {
   Rows r;
   if (const int code = check_rows(in, r); code != NVFP4_OK) return code;
-  if (!old_logp || !advantage || !logp || !lse || !weight || !terms || !loss || !stats2 || !workspace) return NVFP4_E_NULL;
+  if (!old_logp || !advantage || !logp || !stat || !weight || !terms || !loss || !stats2 || !workspace) return NVFP4_E_NULL;
   if (rows_per_advantage <= 0 || rows_per_advantage > 0x7fffffffLL) return NVFP4_E_SHAPE;
   if (workspace_bytes < NVFP4_LOSS_WORKSPACE) return NVFP4_E_WORKSPACE;
-  if (!aligned(old_logp, 4) || !aligned(advantage, 4) || !aligned(ref_logp, 4) || !aligned(logp, 4) || !aligned(lse, 4) ||
+  if (!aligned(old_logp, 4) || !aligned(advantage, 4) || !aligned(ref_logp, 4) || !aligned(logp, 4) || !aligned(stat, 8) ||
       !aligned(weight, 4) || !aligned(terms, 4) || !aligned(loss, 4) || !aligned(stats2, 4) || !aligned(dlogits, in->is_f32 ? 4 : 2) || !aligned(workspace, 16))
     return NVFP4_E_ALIGN;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
@@ -676,7 +684,7 @@ extern "C" int nvfp4_policy_fwd(const nvfp4_logit_rows* in, const float* old_log
   if (const int code = launched(); code != NVFP4_OK) return code;
   const Policy p{old_logp, ref_logp, advantage, (uint32_t)rows_per_advantage, (float)(1.0 - clip_low),
                  (float)(1.0 + clip_high), (float)kl};
-  const PolicyOut o{logp, lse, weight, terms};
+  const PolicyOut o{logp, stat, weight, terms};
   policy_rows(r, in->is_f32 != 0, p, words, counts, o, dlogits, dstride_b, dstride_t, stream);
   if (const int code = launched(); code != NVFP4_OK) return code;
   const int64_t sums = (r.rows + kThreads * 8 - 1) / (kThreads * 8);

@@ -1,0 +1,118 @@
+"""Losses on logits (csrc/logprob.cu, losses.py) at values where a formula that is right for ordinary numbers goes wrong: rows of
+one mask value, common offsets, infinite margins, long sums, arguments of other precision or layout."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+IGNORE = -100
+U = 2.0 ** -24                                     # half a step of fp32
+
+
+@pytest.fixture(scope="module")
+def losses():
+    from nvfp4_sm120_b200 import losses as module
+    return module
+
+
+def _randn(shape, seed, dtype=torch.float32):
+    return torch.randn(shape, device="cuda", dtype=dtype, generator=torch.Generator(device="cuda").manual_seed(seed))
+
+
+def _labels(shape, vocab, seed, masked=0.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed + 1000)
+    y = torch.randint(0, vocab, shape, device="cuda", generator=gen)
+    y[torch.rand(shape, device="cuda", generator=gen) < masked] = IGNORE
+    return y
+
+
+# ---- rows far from zero -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("vocab", [13, 301, 2051, 50257])
+@pytest.mark.parametrize("dtype,step,offsets", [(torch.float32, 1 / 16, (1e4, -1e4, 1e6, -1e6)), (torch.bfloat16, 4.0, (512.0, -512.0))])
+def test_a_common_offset_changes_nothing(losses, vocab, dtype, step, offsets):
+    """Logits on a grid that the offset leaves exact: x - M are the same numbers, and with them every result and gradient."""
+    base = step * torch.randint(-40, 41, (4, 6, vocab), device="cuda", generator=torch.Generator(device="cuda").manual_seed(vocab)).float()
+    y, adv, w = _labels((4, 6), vocab, 1, 0.2), _randn((4,), 2), _randn((4, 6), 3)
+
+    def results(x):
+        x = x.to(dtype).requires_grad_(True)
+        lp = losses.token_logprobs(x, y)
+        pref = losses.preference_loss(x, y, lp.detach().sum(1) + adv)
+        pol = losses.policy_loss(x, y, lp.detach() - 0.05, adv, lp.detach() + 0.1, kl_coef=0.1)
+        grads = [torch.autograd.grad(o, x, g)[0] for o, g in ((lp, w), (pref[0], None), (pol[0], None))]
+        return [lp, *pref, pol[0], *pol[1].values(), *grads]
+
+    want = results(base)
+    for c in offsets:
+        assert ((base + c).to(dtype).double() == base.double() + c).all()
+        assert all(torch.equal(a, b) for a, b in zip(results(base + c), want))
+
+
+@pytest.mark.parametrize("vocab", [1, 13, 2049, 50257])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_one_value(losses, dtype, vocab):
+    """Every logit the same, the type's lowest value (a row whose mask leaves nothing) to its highest: the softmax is 1 / vocab."""
+    info = torch.finfo(dtype)
+    values = torch.tensor([info.min, -1e9, -1e4, 0.0, 1e9, info.max], device="cuda")
+    x = values[:, None].expand(6, vocab).to(dtype).contiguous().requires_grad_(True)
+    y, w = _labels((6,), vocab, 1), _randn((6,), 2)
+    log_v = math.log(vocab)
+    # the sum is exact; logf 2 steps of at most ln 2, the rest of the logarithm in 64 bits, one rounding of the result
+    tol = 2 * U + U * log_v
+    lp = losses.token_logprobs(x, y)
+    assert (lp.double() + log_v).abs().max() <= tol
+    # p: the logarithm's error, its rounding to fp32 in base 2 (times ln 2), ex2.approx 2^-22, two roundings; one to the dtype
+    p = 1 / vocab
+    rel = 2 * U + U * log_v + 2.0 ** -22 + 2 * U
+    hot = torch.zeros(6, vocab, device="cuda", dtype=torch.float64).scatter_(1, y[:, None], 1.0)
+
+    def right(g, w, w_rel=0.0):
+        """w_rel: relative error that w itself may have."""
+        want = w.double()[:, None] * (hot - p)
+        off = w.double().abs()[:, None] * (p * rel + U + w_rel) + info.eps / 2 * 1.001 * want.abs()
+        return ((g.double() - want).abs() <= off).all()
+
+    assert right(torch.autograd.grad(lp, x, w)[0], w)
+    # ratios of 1 and no KL term: dloss / dlogp = -A times a rounded 1 / 6
+    loss, stats = losses.policy_loss(x, y, lp.detach(), w)
+    assert torch.equal(stats["logps"], lp)
+    assert right(torch.autograd.grad(loss, x)[0], -w / 6, 3 * U)
+    # reward margins of 0: dloss / dL = -+ beta / 2 / pairs, and the sigmoid moves by half of itself times the margin's error
+    ref = torch.full((6,), -log_v, device="cuda")
+    off = 2 * (tol + U * log_v)
+    loss, chosen, rejected = losses.preference_loss(x[:, None], y[:, None], ref, beta=1.0)
+    assert torch.cat((chosen, rejected)).abs().max() <= off
+    half = torch.tensor([-1 / 6] * 3 + [1 / 6] * 3, device="cuda")
+    assert right(torch.autograd.grad(loss, x)[0], half, off + 2 * U)
+    assert abs(loss.item() - math.log(2)) <= off + U
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [13, 2049])
+def test_masked_rows(losses, dtype, vocab):
+    """Rows with masked entries, rows whose mask leaves one entry or nothing, a masked label."""
+    x = (3 * _randn((6, vocab), 5)).to(dtype)
+    y = torch.full((6,), 3, device="cuda")
+    low = torch.finfo(dtype).min
+    x[0, 5:] = -math.inf
+    x[1, :] = low
+    x[2, 5:] = low
+    x[3, :] = -math.inf
+    x[3, 3] = 2.0
+    x[4, :] = torch.finfo(dtype).max
+    x[5, 3] = -math.inf
+    x.requires_grad_(True)
+    out = losses.token_logprobs(x, y)
+    lp = out.detach()
+    want = torch.log_softmax(x.detach()[[0, 2]].double(), 1)[:, 3]
+    assert (lp[[0, 2]].double() - want).abs().max() < 2.0 ** -20
+    assert (lp[[1, 4]].double() + math.log(vocab)).abs().max() <= 2 * U + U * math.log(vocab)
+    assert float(lp[3]) == 0.0 and float(lp[5]) == -math.inf
+    (g,) = torch.autograd.grad(out[[0, 2, 3]].sum(), x, retain_graph=True)
+    assert torch.isfinite(g).all() and (g[0, 5:] == 0).all() and (g[2, 5:] == 0).all() and (g[3] == 0).all()
+    assert (g[[1, 4, 5]] == 0).all()                   # nothing was asked of these
+    (g,) = torch.autograd.grad(out[[1, 4]].sum(), x)
+    want = torch.nn.functional.one_hot(y[[1, 4]], vocab).double() - 1 / vocab
+    assert ((g[[1, 4]].double() - want).abs() <= (torch.finfo(dtype).eps + 2.0 ** -20) * want.abs()).all()

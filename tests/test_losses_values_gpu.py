@@ -116,3 +116,20 @@ def test_masked_rows(losses, dtype, vocab):
     (g,) = torch.autograd.grad(out[[1, 4]].sum(), x)
     want = torch.nn.functional.one_hot(y[[1, 4]], vocab).double() - 1 / vocab
     assert ((g[[1, 4]].double() - want).abs() <= (torch.finfo(dtype).eps + 2.0 ** -20) * want.abs()).all()
+
+
+# ---- long sums ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("vocab,spread", [(1000, 2.0), (50257, 4.0), (150000, 4.0)])
+def test_rows_of_a_sequence_are_not_off_the_same_way(losses, vocab, spread):
+    """Most terms of a wide row are below 2^-24 of its sum, and must not vanish from it: a reward adds up a thousand such rows.
+    The mean error of a row, from sequences whose reference is their own sum: ex2.approx is off by 2^-22 at most, the rest are roundings
+    without a sign; those of a row are some 4 U (exponents of the few largest terms, three or so, and the logarithm), so the mean of n
+    rows lies within five times that over sqrt(n)."""
+    n = 640                                          # enough of them that a row gets the fewest threads
+    x = spread * _randn((2, n // 2, vocab), vocab)
+    y = _labels((2, n // 2), vocab, 1)
+    want = torch.stack([torch.log_softmax(s.double(), 1).gather(1, t[:, None]).sum() for s, t in zip(x, y)])
+    ref = want.float()
+    _, chosen, rejected = losses.preference_loss(x, y, ref, beta=1.0)
+    off = (torch.cat((chosen, rejected)).double() + ref.double() - want).sum() / n
+    assert abs(float(off)) <= 2.0 ** -22 + 5 * 4 * U / math.sqrt(n)

@@ -412,7 +412,9 @@ __global__ void __launch_bounds__(kThreads) preference_kernel(const double* __re
     if (threadIdx.x == 0) {
       const double chosen = beta * (s[0] - ref[p]), rejected = beta * (s[1] - ref[pairs + p]), h = chosen - rejected;
       const double tail = log1p(exp(-fabs(h)));             // -logsigmoid(h) = max(-h, 0) + log(1 + exp(-|h|))
-      sum[0] += (1.0 - smooth) * (fmax(-h, 0.0) + tail) + smooth * (fmax(h, 0.0) + tail);
+      // (h is infinite where a label's logit is -inf; a term whose factor is 0 is left out then, not 0 times infinity)
+      if (smooth < 1.0) sum[0] += (1.0 - smooth) * (fmax(-h, 0.0) + tail);
+      if (smooth > 0.0) sum[0] += smooth * (fmax(h, 0.0) + tail);
       if (h != h) sum[0] = h;
       const double w = beta / (double)pairs * (smooth / (1.0 + exp(-h)) - (1.0 - smooth) / (1.0 + exp(h)));
       rewards[p] = (float)chosen;

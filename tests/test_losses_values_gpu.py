@@ -133,3 +133,39 @@ def test_rows_of_a_sequence_are_not_off_the_same_way(losses, vocab, spread):
     _, chosen, rejected = losses.preference_loss(x, y, ref, beta=1.0)
     off = (torch.cat((chosen, rejected)).double() + ref.double() - want).sum() / n
     assert abs(float(off)) <= 2.0 ** -22 + 5 * 4 * U / math.sqrt(n)
+
+
+# ---- infinite margins ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("smooth", [0.0, 0.1, 1.0])
+def test_preference_with_an_impossible_token(losses, dtype, smooth):
+    """A label whose logit is -inf makes its sequence's sum -inf: in a rejected sequence h = inf, where -logsigmoid(h) is 0, in a chosen
+    one h = -inf, where it is inf.  The other pairs count as ever."""
+    P, T, V = 3, 5, 17
+    y, ref = _labels((2 * P, T), V, 2), _randn((2 * P,), 3) - T * math.log(V)
+    for impossible in (P + 1, 1):                      # of the middle pair: the rejected sequence, the chosen one
+        x = (0.3 * _randn((2 * P, T, V), 4)).to(dtype)
+        x[impossible, 2, y[impossible, 2]] = -math.inf
+        x.requires_grad_(True)
+        loss, chosen, rejected = losses.preference_loss(x, y, ref, beta=0.5, label_smoothing=smooth)
+        L = torch.log_softmax(x.detach().double(), 2).gather(2, y[..., None])[..., 0].sum(1)
+        c, r = (0.5 * (L - ref.double())).chunk(2)
+        h = c - r
+        softplus = lambda t: torch.nn.functional.softplus(t.double())
+        terms = torch.zeros_like(h)
+        if smooth < 1:
+            terms += (1 - smooth) * softplus(-h)
+        if smooth > 0:
+            terms += smooth * softplus(h)
+        want = terms.mean().item()
+        assert torch.equal(torch.isinf(torch.cat((chosen, rejected))), torch.isinf(torch.cat((c, r))))
+        # five log-probabilities of some 3, their rewards, the loss: a few dozen roundings
+        assert loss.item() == want if math.isinf(want) else abs(loss.item() - want) <= 64 * U * (1 + want)
+        (g,) = torch.autograd.grad(loss, x)
+        assert torch.isfinite(g).all()
+        # dloss / dL: beta / P (s sigmoid(h) - (1 - s) sigmoid(-h)), 0 or a constant where h is infinite
+        w = 0.5 / P * (smooth * torch.sigmoid(h) - (1 - smooth) * torch.sigmoid(-h))
+        w = torch.cat((w, -w))[:, None, None]
+        hot = torch.nn.functional.one_hot(y, V).double()
+        exact = w * (hot - torch.softmax(x.detach().double(), 2))
+        assert ((g.double() - exact).abs() <= (torch.finfo(dtype).eps / 2 + 64 * U) * exact.abs() + 64 * U * w.abs()).all()

@@ -473,7 +473,7 @@ int nvfp4_preference_fwd(const nvfp4_logit_rows* rows, const float* ref, double 
 /*
  * Clipped policy loss with a KL term: rho = exp(logp - old_logp), A = advantage[row / rows_per_advantage], d = ref_logp - logp,
  * loss = 1/n sum over the n rows with a label (n = 1 if there are none) of
- *   -min(rho A, clamp(rho, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1)     (no KL term when ref_logp is NULL)
+ *   -min(rho A, clamp(rho, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1)     (no KL term when ref_logp is NULL or kl is 0)
  * stats2 = {mean of exp(d) - d - 1, share of rows whose clamp cut the gradient}; weight[row] = dloss / dlogp.
  * terms: scratch [2, batch * seq].  dlogits: NULL, or the gradient of the loss in nvfp4_logprob_bwd's layout, written while the row is on chip.
  * No counterpart in the reference.

@@ -488,18 +488,21 @@ __device__ __forceinline__ float policy_row(const Policy& p, const PolicyOut& o,
   const float a = in.advantage, rho = expf(logp - in.old);
   const float s = rho * a, q = fminf(fmaxf(rho, p.low), p.high) * a;
   const bool clipped = s > q;                                // (not when it is no number: that has to show)
-  float w = clipped ? 0.0f : -s, kl = 0.0f;
+  float w = clipped ? 0.0f : -s, kl = 0.0f, term = -(clipped ? q : s);
   if (p.ref != nullptr) {
     const float d = in.ref - logp, e = expm1f(d);
-    kl = fabsf(e - d);                                       // (never negative but for the last rounding)
-    w = fmaf(-p.kl, e, w);
+    kl = e <= FLT_MAX ? fabsf(e - d) : e;                    // (never negative but for the last rounding; inf - inf is inf here)
+    if (p.kl != 0.0f) {                                      // (the term may be infinite where it is only looked at)
+      w = fmaf(-p.kl, e, w);
+      term = fmaf(p.kl, kl, term);
+    }
   }
   w *= share;
   if (store) {
     o.logp[row] = logp;
     o.norm[row] = norm;
     o.weight[row] = w;
-    o.term[row] = fmaf(p.kl, kl, -(clipped ? q : s));
+    o.term[row] = term;
     o.term[rows + row] = clipped ? -kl : kl;
   }
   return w;

@@ -38,7 +38,7 @@ def policy_loss(logits, labels, old_logps, advantages, ref_logps=None, clip=0.2,
     """Clipped policy loss with a KL term, (loss, stats).
 
     old_logps: log-probabilities of the labels when they were sampled; advantages: one per sequence [batch] or one per
-    label; ref_logps: log-probabilities under the reference model, for the KL term.  With rho = exp(logp - old) and
+    label; ref_logps: log-probabilities under the reference model, for the KL term (with kl_coef 0 for `kl` alone).  With rho = exp(logp - old) and
     d = ref - logp, the loss is the mean over all labels that are not ignored (0 if there are none) of
     -min(rho A, clamp(rho, 1 - clip, 1 + clip_high) A) + kl_coef (exp(d) - d - 1); clip_high None means clip.
     stats: `logps` (of the labels' shape, 0 where ignored), `kl` (mean of exp(d) - d - 1) and `clip_fraction`.

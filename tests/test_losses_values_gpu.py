@@ -169,3 +169,22 @@ def test_preference_with_an_impossible_token(losses, dtype, smooth):
         hot = torch.nn.functional.one_hot(y, V).double()
         exact = w * (hot - torch.softmax(x.detach().double(), 2))
         assert ((g.double() - exact).abs() <= (torch.finfo(dtype).eps / 2 + 64 * U) * exact.abs() + 64 * U * w.abs()).all()
+
+
+# ---- a reference that is only looked at ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_reference_without_a_coefficient_leaves_the_loss_alone(losses, dtype):
+    """kl_coef 0: `kl` is measured, and the loss and its gradient are those of a call without a reference, however far that lies."""
+    x = (2 * _randn((3, 4, 19), 1)).to(dtype).requires_grad_(True)
+    y, adv = _labels((3, 4), 19, 2, 0.2), _randn((3,), 3)
+    y[0, 0] = 3
+    lp = losses.token_logprobs(x, y).detach()
+    old = lp - 0.1
+    plain, without = losses.policy_loss(x, y, old, adv)
+    (g,) = torch.autograd.grad(plain, x)
+    for far, kl in ((0.3, math.exp(0.3) - 1.3), (200.0, math.inf), (math.inf, math.inf)):
+        loss, stats = losses.policy_loss(x, y, old, adv, lp + far)
+        (h,) = torch.autograd.grad(loss, x)
+        assert torch.equal(loss, plain) and torch.equal(h, g) and torch.equal(stats["clip_fraction"], without["clip_fraction"])
+        # ref - logp is off by a rounding of ref, some 2^-21, and its term by that times exp(0.3) - 1
+        assert float(stats["kl"]) == kl if math.isinf(kl) else abs(float(stats["kl"]) - kl) <= 2.0 ** -21

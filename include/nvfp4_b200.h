@@ -427,7 +427,7 @@ int nvfp4_norm_of_sumsq(const double* parts, int n_parts, float* norm, void* str
  * Losses on logits [batch, seq, vocab] (fp32, or bf16 when is_f32 == 0; strides in elements, the logits of a row contiguous;
  * rows are numbered batch * seq + position).  A row whose label equals ignore_index has no part in anything and is not read;
  * any other label outside [0, vocab) gives NaN.  At most 2^31 - 1 rows of at most 2^31 - 1 logits.  All row and sequence
- * vectors are fp32.
+ * vectors are fp32 where nothing else is said.
  */
 typedef struct {
   const void* logits;
@@ -461,12 +461,12 @@ int nvfp4_logprob_bwd(const nvfp4_logit_rows* rows, const nvfp4_row_stat* stat, 
 
 /*
  * Preference loss of batch / 2 pairs, sequence i chosen over sequence batch / 2 + i: with L_i the sum of the sequence's
- * logp (fp64 here, [batch * seq]: a reward is a small difference of long sums),
+ * logp (fp64 here, [batch * seq], as ref [batch] is: a reward is a small difference of long sums),
  * rewards[i] = beta (L_i - ref[i]), h = rewards[chosen] - rewards[rejected],
  * loss = mean(-(1 - label_smoothing) logsigmoid(h) - label_smoothing logsigmoid(-h)).
  * weight[i] = dloss / dL_i, for nvfp4_logprob_bwd with rows_per_weight = seq.  No counterpart in the reference.
  */
-int nvfp4_preference_fwd(const nvfp4_logit_rows* rows, const float* ref, double beta, double label_smoothing, double* logp,
+int nvfp4_preference_fwd(const nvfp4_logit_rows* rows, const double* ref, double beta, double label_smoothing, double* logp,
                          nvfp4_row_stat* stat, float* loss, float* rewards, float* weight, void* workspace, size_t workspace_bytes,
                          void* stream);
 

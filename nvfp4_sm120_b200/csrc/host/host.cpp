@@ -662,10 +662,10 @@ struct Logits {
   int64_t count() const { return rows.batch * rows.seq; }
   at::Tensor per_row() const { return at::empty(labels.sizes(), on(dev, at::kFloat)); }
   // a row or sequence vector as the kernels read it
-  at::Tensor vec(const at::Tensor& t, int64_t n, const char* name) const {
+  at::Tensor vec(const at::Tensor& t, int64_t n, const char* name, at::ScalarType type = at::kFloat) const {
     device_of({&x, &t});
     if (t.numel() != n || !t.is_floating_point()) raise(PyExc_ValueError, std::string(name) + " must hold " + std::to_string(n) + " floating-point values");
-    return t.to(at::kFloat).contiguous();
+    return t.to(type).contiguous();
   }
 };
 
@@ -745,14 +745,14 @@ struct Preference : torch::autograd::Function<Preference> {
     const Logits in(logits, labels, ignore);
     if (logits.dim() != 3 || in.rows.batch % 2 != 0)
       raise(PyExc_ValueError, "logits must be [2 pairs, seq, vocab], the chosen sequences first");
-    const at::Tensor r = in.vec(ref, in.rows.batch, "ref_logps");
+    const at::Tensor r = in.vec(ref, in.rows.batch, "ref_logps", at::kDouble);
     const c10::cuda::CUDAGuard guard(in.dev);
     const int64_t n = in.count();
     at::Tensor loss = at::empty({}, on(in.dev, at::kFloat)), rewards = at::empty({in.rows.batch}, on(in.dev, at::kFloat)),
                kept = at::empty({2 * n + in.rows.batch}, on(in.dev, at::kFloat));
     const at::Tensor scratch = loss_scratch(in.dev, 8 * n);
     uint8_t* ws = scratch.data_ptr<uint8_t>();
-    check(lib.nvfp4_preference_fwd(&in.rows, float_ptr(r), beta, smoothing, reinterpret_cast<double*>(ws + NVFP4_LOSS_WORKSPACE),
+    check(lib.nvfp4_preference_fwd(&in.rows, r.data_ptr<double>(), beta, smoothing, reinterpret_cast<double*>(ws + NVFP4_LOSS_WORKSPACE),
                                    stat_ptr(kept), float_ptr(loss), float_ptr(rewards), float_ptr(kept) + 2 * n, ws, NVFP4_LOSS_WORKSPACE,
                                    stream_of(in.dev)),
           "nvfp4_preference_fwd");

@@ -397,7 +397,7 @@ template <int N> __device__ __forceinline__ bool grid_sum(double (&v)[N], double
 
 // ---- preference loss ----------------------------------------------------------------------------------------------------
 // One CTA per pair in turn: sums of both sequences in 64 bits (they differ little and are long), rewards, loss, weights.
-__global__ void __launch_bounds__(kThreads) preference_kernel(const double* __restrict__ logp, const float* __restrict__ ref, int64_t pairs,
+__global__ void __launch_bounds__(kThreads) preference_kernel(const double* __restrict__ logp, const double* __restrict__ ref, int64_t pairs,
                                                               uint32_t seq, double beta, double smooth, double* __restrict__ parts,
                                                               unsigned int* __restrict__ ticket, float* __restrict__ loss,
                                                               float* __restrict__ rewards, float* __restrict__ weight) {
@@ -658,7 +658,7 @@ extern "C" int nvfp4_logprob_bwd(const nvfp4_logit_rows* in, const nvfp4_row_sta
   return launched();
 }
 
-extern "C" int nvfp4_preference_fwd(const nvfp4_logit_rows* in, const float* ref, double beta, double label_smoothing, double* logp,
+extern "C" int nvfp4_preference_fwd(const nvfp4_logit_rows* in, const double* ref, double beta, double label_smoothing, double* logp,
                                     nvfp4_row_stat* stat, float* loss, float* rewards, float* weight, void* workspace,
                                     size_t workspace_bytes, void* stream_) {
   Rows r;
@@ -666,7 +666,7 @@ extern "C" int nvfp4_preference_fwd(const nvfp4_logit_rows* in, const float* ref
   if (in->batch % 2 != 0) return NVFP4_E_SHAPE;
   if (!ref || !logp || !stat || !loss || !rewards || !weight || !workspace) return NVFP4_E_NULL;
   if (workspace_bytes < NVFP4_LOSS_WORKSPACE) return NVFP4_E_WORKSPACE;
-  if (!aligned(ref, 4) || !aligned(logp, 8) || !aligned(stat, 8) || !aligned(loss, 4) || !aligned(rewards, 4) || !aligned(weight, 4) ||
+  if (!aligned(ref, 8) || !aligned(logp, 8) || !aligned(stat, 8) || !aligned(loss, 4) || !aligned(rewards, 4) || !aligned(weight, 4) ||
       !aligned(workspace, 16))
     return NVFP4_E_ALIGN;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);

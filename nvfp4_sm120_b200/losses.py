@@ -25,7 +25,8 @@ def preference_loss(logits, labels, ref_logps, beta=0.1, label_smoothing=0.0, ig
     """Loss over pairs of sequences, (loss, chosen rewards [pairs], rejected rewards [pairs]).
 
     logits [2 pairs, seq, vocab]: sequence i was preferred to sequence pairs + i.  ref_logps [2 pairs]: the sums of the
-    sequences' log-probabilities under the reference model.  With L_i the sum of sequence i's log-probabilities,
+    sequences' log-probabilities under the reference model, best in 64 bits (token_logprobs(...).double().sum(1)): a reward is a
+    small difference of long sums, and fp32 alone rounds a sum of 5000 by 2e-4.  With L_i the sum of sequence i's log-probabilities,
     reward_i = beta (L_i - ref_i) and h = reward_chosen - reward_rejected, the loss is the mean over the pairs of
     -(1 - label_smoothing) logsigmoid(h) - label_smoothing logsigmoid(-h)."""
     if not 0.0 <= label_smoothing <= 1.0:

@@ -188,3 +188,21 @@ def test_reference_without_a_coefficient_leaves_the_loss_alone(losses, dtype):
         assert torch.equal(loss, plain) and torch.equal(h, g) and torch.equal(stats["clip_fraction"], without["clip_fraction"])
         # ref - logp is off by a rounding of ref, some 2^-21, and its term by that times exp(0.3) - 1
         assert float(stats["kl"]) == kl if math.isinf(kl) else abs(float(stats["kl"]) - kl) <= 2.0 ** -21
+
+
+# ---- references in 64 bits ----------------------------------------------------------------------------------------------
+def test_reference_sums_keep_their_precision(losses):
+    """The reference of sequences of thousands of nats, in 64 bits: rewards are the small differences they are made of."""
+    x = 2 * _randn((4, 1500, 301), 1)
+    y = _labels((4, 1500), 301, 2)
+    ref = losses.token_logprobs(x, y).double().sum(1)
+    assert ref.abs().min() > 8192
+    for shift in (0.0, 2.0 ** -13):                    # an eighth of an fp32 step there
+        _, chosen, rejected = losses.preference_loss(x, y, ref + shift, beta=1.0)
+        got = torch.cat((chosen, rejected)).double()
+        # the same log-probabilities before and behind their rounding to fp32, of at most 2^-20 (under 32) and without a sign: five
+        # standard deviations of the sum of 1500
+        assert (got + shift).abs().max() <= 5 * 2.0 ** -20 / math.sqrt(3 / 1500)
+    ints = torch.arange(4, device="cuda")
+    with pytest.raises(ValueError, match="floating"):
+        losses.preference_loss(x, y, ints)

@@ -59,6 +59,7 @@ void check(int code, const char* what) {
 }
 
 [[noreturn]] void raise(PyObject* type, const std::string& msg) {
+  if (!PyGILState_Check()) throw std::runtime_error(msg);      // a node of the backward pass, on autograd's thread
   PyErr_SetString(type, msg.c_str());
   throw py::error_already_set();
 }
@@ -77,6 +78,7 @@ c10::Device device_of(std::initializer_list<const at::Tensor*> ts) {
     dev = t->device();
   }
   if (!good || !dev.has_value()) {
+    if (!PyGILState_Check()) throw std::runtime_error("operands are not on one CUDA device");
     py::list l;
     for (const at::Tensor* t : ts) {
       if (t == nullptr) l.append(py::none());
@@ -701,19 +703,24 @@ void only_once(const tensor_list& grads) {
 }
 nvfp4_row_stat* stat_ptr(const at::Tensor& t) { return reinterpret_cast<nvfp4_row_stat*>(float_ptr(t)); }
 // Gradient of the logits.  saved: logits, labels and, in one tensor, the rows' statistics and dloss / dlogp (one per row or per
-// sequence), or the former alone and `weight` for the latter; scale: what dloss / dlogp is to be multiplied with (one
+// sequence, `per` rows each), or the former alone and `weight` for the latter.  They come back as a hook on saved tensors or an
+// assignment to their .data left them, and are looked at again.  scale: what dloss / dlogp is to be multiplied with (one
 // element); ready: the gradient for a scale of 1, used again where the scale is 1
-at::Tensor dlogits(const torch::autograd::variable_list& saved, int64_t ignore, const at::Tensor& weight, const at::Tensor& scale,
-                   const at::Tensor& ready) {
+at::Tensor dlogits(const torch::autograd::variable_list& saved, int64_t ignore, int64_t per, const at::Tensor& weight,
+                   const at::Tensor& scale, const at::Tensor& ready) {
   const Logits in(saved[0], saved[1], ignore);
   const c10::cuda::CUDAGuard guard(in.dev);
   const int64_t n = in.count();
-  const at::Tensor w = weight.defined() ? weight.to(at::kFloat).contiguous() : saved[2],
+  const at::Tensor& kept = saved[2];
+  if (kept.device() != in.dev || kept.scalar_type() != at::kFloat || !kept.is_contiguous() || kept.is_neg() || n % per != 0 ||
+      kept.numel() != 2 * n + (weight.defined() ? 0 : n / per) || reinterpret_cast<uintptr_t>(kept.data_ptr()) % 8 != 0 ||
+      (ready.defined() && (ready.sizes() != in.x.sizes() || ready.scalar_type() != in.x.scalar_type())))
+    throw std::runtime_error("what a loss saved for its backward pass came back changed");
+  const at::Tensor w = weight.defined() ? weight.to(at::kFloat).contiguous() : kept,
                    sc = scale.defined() ? scale.to(at::kFloat) : scale;
   const float* wp = float_ptr(w) + (weight.defined() ? 0 : 2 * n);
-  const int64_t per = n / (weight.defined() ? n : saved[2].numel() - 2 * n);
   at::Tensor out = ready.defined() ? ready : gradient_like(saved[0], in);
-  check_in_backward(lib.nvfp4_logprob_bwd(&in.rows, stat_ptr(saved[2]), wp, per, sc.defined() ? float_ptr(sc) : nullptr,
+  check_in_backward(lib.nvfp4_logprob_bwd(&in.rows, stat_ptr(kept), wp, per, sc.defined() ? float_ptr(sc) : nullptr,
                                           ready.defined(), out.data_ptr(), batch_stride(out), out.stride(-2), stream_of(in.dev)),
                     "nvfp4_logprob_bwd");
   return out;
@@ -731,7 +738,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
     only_once(grads);
-    return {dlogits(ctx->get_saved_variables(), ctx->saved_data["ignore"].toInt(), grads[0], {}, {}), {}, {}};
+    return {dlogits(ctx->get_saved_variables(), ctx->saved_data["ignore"].toInt(), 1, grads[0], {}, {}), {}, {}};
   }
 };
 
@@ -758,6 +765,7 @@ struct Preference : torch::autograd::Function<Preference> {
           "nvfp4_preference_fwd");
     ctx->save_for_backward({logits, labels, kept});
     ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["seq"] = in.rows.seq;
     ctx->mark_non_differentiable({rewards});
     ctx->set_materialize_grads(false);
     return {loss, rewards};
@@ -765,7 +773,8 @@ struct Preference : torch::autograd::Function<Preference> {
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
     only_once(grads);
     if (!grads[0].defined()) return tensor_list(6);          // the node behind this one gave no gradient
-    return {dlogits(ctx->get_saved_variables(), ctx->saved_data["ignore"].toInt(), {}, grads[0], {}), {}, {}, {}, {}, {}};
+    return {dlogits(ctx->get_saved_variables(), ctx->saved_data["ignore"].toInt(), ctx->saved_data["seq"].toInt(), {}, grads[0], {}),
+            {}, {}, {}, {}, {}};
   }
 };
 
@@ -809,7 +818,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
       ready = it->second.toTensor();
       ctx->saved_data.erase(it);
     }
-    return {dlogits(ctx->get_saved_variables(), ctx->saved_data["ignore"].toInt(), {}, grads[0], ready), {}, {}, {}, {}, {}, {}, {}, {}, {}};
+    return {dlogits(ctx->get_saved_variables(), ctx->saved_data["ignore"].toInt(), 1, {}, grads[0], ready), {}, {}, {}, {}, {}, {}, {}, {}, {}};
   }
 };
 

@@ -1,0 +1,74 @@
+"""Losses on logits (losses.py) as nodes of an autograd graph: hooks on saved tensors, second derivatives, what may have changed
+between the forward and the backward pass."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+IGNORE = -100
+
+
+@pytest.fixture(scope="module")
+def losses():
+    from nvfp4_sm120_b200 import losses as module
+    return module
+
+
+def _randn(shape, seed, dtype=torch.float32):
+    return torch.randn(shape, device="cuda", dtype=dtype, generator=torch.Generator(device="cuda").manual_seed(seed))
+
+
+def _data(shape=(4, 6, 83), seed=1):
+    """logits, labels, a vector of a value for each sequence and one for each label"""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    y = torch.randint(0, shape[-1], shape[:-1], device="cuda", generator=gen)
+    y[torch.rand(shape[:-1], device="cuda", generator=gen) < 0.3] = IGNORE
+    return _randn(shape, seed), y, _randn(shape[:1], seed + 1), -4 + 0.3 * _randn(shape[:-1], seed + 2)
+
+
+def _calls(losses, y, per_sequence, per_label):
+    """Each loss as a function of the logits alone, with a gradient that all of its elements count in."""
+    w = _randn(y.shape, 9)
+    return {"logprobs": lambda x: (losses.token_logprobs(x, y) * w).sum(),
+            "preference": lambda x: losses.preference_loss(x, y, per_sequence)[0],
+            "policy": lambda x: losses.policy_loss(x, y, per_label, per_sequence, per_label + 0.1, kl_coef=0.1)[0]}
+
+
+NAMES = ["logprobs", "preference", "policy"]
+
+
+# ---- what was saved -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("name", NAMES)
+def test_saved_tensors_that_come_back_changed_are_refused(losses, name):
+    x, y, a, b = _data()
+    call = _calls(losses, y, a, b)[name]
+    x.requires_grad_(True)
+    (want,) = torch.autograd.grad(call(x), x)
+    same = lambda t: t
+    vector = lambda t: t.dim() == 1 and t.is_floating_point()
+    for unpack in (lambda t: t.half() if vector(t) else t, lambda t: t[:-1] if vector(t) else t, lambda t: t[:0] if vector(t) else t,
+                   lambda t: t.cpu(), lambda t: t.cpu() if vector(t) else t, lambda t: t.cpu() if t.dim() == 2 else t,
+                   lambda t: t.half() if t.dim() == 3 else t, lambda t: torch.cat((t, t), -1) if t.dim() == 3 else t, lambda t: t.float() if t.dim() == 2 else t,
+                   lambda t: t[:, :-1] if t.dim() == 3 else t, lambda t: t[:, :-1] if t.dim() > 1 else t,
+                   lambda t: torch.cat((t, t)) if t.dim() > 1 else t, lambda t: t[:1].expand(t.shape) if vector(t) else t):
+        with torch.autograd.graph.saved_tensors_hooks(same, unpack):
+            loss = call(x)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(3 * loss, x)           # (a factor: the policy loss has to write its gradient again)
+    assert torch.equal(torch.autograd.grad(call(x), x)[0], want)
+    with torch.autograd.graph.save_on_cpu():
+        loss = call(x)
+    assert torch.equal(torch.autograd.grad(loss, x)[0], want)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_logits_swapped_behind_autograds_back_are_refused(losses, name):
+    for other in (lambda x: x[:, :3].clone(), lambda x: torch.cat((x, x)), lambda x: torch.cat((x, x), -1), lambda x: x.bfloat16(), lambda x: x.double(), lambda x: x[0, 0].clone()):
+        x, y, a, b = _data()
+        leaf = x.requires_grad_(True)
+        loss = _calls(losses, y, a, b)[name](leaf)
+        leaf.data = other(leaf.detach())
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(3 * loss, leaf)        # (a factor: the policy loss has to write its gradient again)

@@ -696,11 +696,12 @@ using torch::autograd::tensor_list;
 void check_in_backward(int code, const char* what) {         // without the interpreter
   if (code != 0) throw std::runtime_error(std::string(what) + " failed: " + lib.nvfp4_status_string(code));
 }
-void only_once(const tensor_list& grads) {
-  if (!c10::GradMode::is_enabled()) return;
-  for (const at::Tensor& g : grads)
-    if (g.defined() && g.requires_grad()) throw std::runtime_error("the losses on logits are differentiable once");
-}
+// A gradient that says so when it is differentiated again: it depends on the logits and on the gradient behind it, and without
+// a node of its own a penalty on it would be lost without a word.
+struct Once : torch::autograd::Function<Once> {
+  static at::Tensor forward(AutogradContext*, const at::Tensor& gradient, const at::Tensor&, const at::Tensor&) { return gradient.detach(); }
+  static tensor_list backward(AutogradContext*, tensor_list) { throw std::runtime_error("the losses on logits are differentiable once"); }
+};
 nvfp4_row_stat* stat_ptr(const at::Tensor& t) { return reinterpret_cast<nvfp4_row_stat*>(float_ptr(t)); }
 // Gradient of the logits.  saved: logits, labels and, in one tensor, the rows' statistics and dloss / dlogp (one per row or per
 // sequence, `per` rows each), or the former alone and `weight` for the latter.  They come back as a hook on saved tensors or an
@@ -723,7 +724,7 @@ at::Tensor dlogits(const torch::autograd::variable_list& saved, int64_t ignore, 
   check_in_backward(lib.nvfp4_logprob_bwd(&in.rows, stat_ptr(kept), wp, per, sc.defined() ? float_ptr(sc) : nullptr,
                                           ready.defined(), out.data_ptr(), batch_stride(out), out.stride(-2), stream_of(in.dev)),
                     "nvfp4_logprob_bwd");
-  return out;
+  return c10::GradMode::is_enabled() ? Once::apply(out, saved[0], weight.defined() ? weight : scale) : out;
 }
 
 struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
@@ -737,7 +738,6 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     return logp;
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
-    only_once(grads);
     return {dlogits(ctx->get_saved_variables(), ctx->saved_data["ignore"].toInt(), 1, grads[0], {}, {}), {}, {}};
   }
 };
@@ -771,7 +771,6 @@ struct Preference : torch::autograd::Function<Preference> {
     return {loss, rewards};
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
-    only_once(grads);
     if (!grads[0].defined()) return tensor_list(6);          // the node behind this one gave no gradient
     return {dlogits(ctx->get_saved_variables(), ctx->saved_data["ignore"].toInt(), ctx->saved_data["seq"].toInt(), {}, grads[0], {}),
             {}, {}, {}, {}, {}};
@@ -811,7 +810,6 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     return {loss, stats, logp};
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
-    only_once(grads);
     if (!grads[0].defined()) return tensor_list(10);
     at::Tensor ready;
     if (auto it = ctx->saved_data.find("grad"); it != ctx->saved_data.end()) {      // (a second backward writes its own)

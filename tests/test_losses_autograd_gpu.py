@@ -72,3 +72,34 @@ def test_logits_swapped_behind_autograds_back_are_refused(losses, name):
         leaf.data = other(leaf.detach())
         with pytest.raises(RuntimeError):
             torch.autograd.grad(3 * loss, leaf)        # (a factor: the policy loss has to write its gradient again)
+
+
+# ---- second derivatives -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("name", NAMES)
+def test_second_derivatives_are_refused_not_lost(losses, name):
+    """A penalty on the gradient, added to something that is differentiable: its part must not be left out in silence."""
+    h, y, a, b = _data()
+    call = _calls(losses, y, a, b)[name]
+    head = torch.nn.Parameter(1 + 0.1 * _randn(h.shape[-1:], 5))
+    scale = torch.nn.Parameter(torch.ones((), device="cuda"))
+    for factor in (1.0, scale):
+        x = h * head
+        loss = factor * call(x)
+        (plain,) = torch.autograd.grad(loss, x, retain_graph=True)
+        (g,) = torch.autograd.grad(loss, x, create_graph=True)
+        assert torch.equal(g, plain) and g.requires_grad
+        penalty = g.square().sum()
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(head.sum() + penalty, head, retain_graph=True)
+        if factor is scale:                            # (the other penalty does not depend on it)
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                torch.autograd.grad(head.sum() + scale + penalty, scale, retain_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            (loss + penalty).backward()
+    head.grad = None                                   # without a second derivative such a graph is as good as any
+    (call(h * head) + 0.0).backward(create_graph=True)
+    first = head.grad.detach().clone()
+    head.grad = None
+    call(h * head).backward()
+    assert torch.equal(first, head.grad)
+    head.grad = None

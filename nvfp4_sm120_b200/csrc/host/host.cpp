@@ -17,6 +17,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "nvfp4_b200.h"
@@ -671,6 +672,13 @@ struct Logits {
   }
 };
 
+// Do rows of these strides lie apart?
+bool rows_apart(const nvfp4_logit_rows& r, int64_t stride_b, int64_t stride_t) {
+  const bool time_inside = stride_t <= stride_b || r.batch == 1;
+  const int64_t inner = time_inside ? stride_t : stride_b, outer = time_inside ? stride_b : stride_t;
+  const int64_t n_inner = time_inside ? r.seq : r.batch, n_outer = time_inside ? r.batch : r.seq;
+  return (n_inner == 1 || inner >= r.vocab) && (n_outer == 1 || outer >= (n_inner - 1) * inner + r.vocab);
+}
 // A tensor for the gradient of logits whose rows lie as the logits' own do, modulo 16 bytes: then both are read and written in
 // whole vectors.  (A view of shifted logits has rows at other places than a contiguous tensor of its shape.)
 at::Tensor gradient_like(const at::Tensor& x, const Logits& in) {
@@ -678,11 +686,10 @@ at::Tensor gradient_like(const at::Tensor& x, const Logits& in) {
   const bool time_inside = r.stride_t <= r.stride_b || r.batch == 1;
   const int64_t inner = time_inside ? r.stride_t : r.stride_b, outer = time_inside ? r.stride_b : r.stride_t;
   const int64_t n_inner = time_inside ? r.seq : r.batch, n_outer = time_inside ? r.batch : r.seq;
-  const bool apart = (n_inner == 1 || inner >= r.vocab) && (n_outer == 1 || outer >= (n_inner - 1) * inner + r.vocab);
   const int64_t span = (n_outer - 1) * outer + (n_inner - 1) * inner + r.vocab;
   const int64_t shift = (int64_t)(reinterpret_cast<uintptr_t>(r.logits) % 16) / (r.is_f32 ? 4 : 2);
   const auto opt = on(in.dev, x.scalar_type());
-  if (!apart || !in.x.is_same(x) || span > 2 * x.numel()) return at::empty(x.sizes(), opt);
+  if (!rows_apart(r, r.stride_b, r.stride_t) || !in.x.is_same(x) || span > 2 * x.numel()) return at::empty(x.sizes(), opt);
   if (shift == 0 && x.is_contiguous()) return at::empty(x.sizes(), opt);
   return at::empty({span + shift}, opt).as_strided(x.sizes(), x.strides(), shift);
 }
@@ -715,12 +722,14 @@ at::Tensor dlogits(const torch::autograd::variable_list& saved, int64_t ignore, 
   const at::Tensor& kept = saved[2];
   if (kept.device() != in.dev || kept.scalar_type() != at::kFloat || !kept.is_contiguous() || kept.is_neg() || n % per != 0 ||
       kept.numel() != 2 * n + (weight.defined() ? 0 : n / per) || reinterpret_cast<uintptr_t>(kept.data_ptr()) % 8 != 0 ||
-      (ready.defined() && (ready.sizes() != in.x.sizes() || ready.scalar_type() != in.x.scalar_type())))
+      (ready.defined() && (ready.sizes() != in.x.sizes() || ready.scalar_type() != in.x.scalar_type() || ready.device() != in.dev)))
     throw std::runtime_error("what a loss saved for its backward pass came back changed");
   const at::Tensor w = weight.defined() ? weight.to(at::kFloat).contiguous() : kept,
                    sc = scale.defined() ? scale.to(at::kFloat) : scale;
   const float* wp = float_ptr(w) + (weight.defined() ? 0 : 2 * n);
-  at::Tensor out = ready.defined() ? ready : gradient_like(saved[0], in);
+  at::Tensor out = ready.defined() ? ready.resolve_neg() : gradient_like(saved[0], in);
+  if (ready.defined() && ((out.size(-1) > 1 && out.stride(-1) != 1) || !rows_apart(in.rows, batch_stride(out), out.stride(-2))))
+    out = out.contiguous();                                  // (a hook laid it out anew)
   check_in_backward(lib.nvfp4_logprob_bwd(&in.rows, stat_ptr(kept), wp, per, sc.defined() ? float_ptr(sc) : nullptr,
                                           ready.defined(), out.data_ptr(), batch_stride(out), out.stride(-2), stream_of(in.dev)),
                     "nvfp4_logprob_bwd");
@@ -777,6 +786,13 @@ struct Preference : torch::autograd::Function<Preference> {
   }
 };
 
+// A tensor that waits for the backward pass by itself: hooks on saved tensors see it like any other, and it is let go when it is
+// taken, whether or not the rest of the graph is kept.
+struct Waiting : torch::CustomClassHolder {
+  torch::autograd::SavedVariable tensor;
+  explicit Waiting(const at::Tensor& t) : tensor(t, false) {}
+};
+
 // -> loss, stats, log-probabilities.  The forward kernel writes the gradient for dloss = 1 while it has the rows at hand;
 // the backward writes it again only where the loss arrives with another factor.
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
@@ -804,7 +820,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
           "nvfp4_policy_fwd");
     ctx->save_for_backward({logits, labels, kept});
     ctx->saved_data["ignore"] = ignore;
-    if (want_grad) ctx->saved_data["grad"] = grad;
+    if (want_grad) ctx->saved_data["grad"] = at::IValue::make_capsule(c10::make_intrusive<Waiting>(grad));
     ctx->mark_non_differentiable({stats, logp});
     ctx->set_materialize_grads(false);
     return {loss, stats, logp};
@@ -813,8 +829,9 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     if (!grads[0].defined()) return tensor_list(10);
     at::Tensor ready;
     if (auto it = ctx->saved_data.find("grad"); it != ctx->saved_data.end()) {      // (a second backward writes its own)
-      ready = it->second.toTensor();
+      const auto waiting = it->second.toCapsule();
       ctx->saved_data.erase(it);
+      ready = static_cast<Waiting*>(waiting.get())->tensor.unpack();
     }
     return {dlogits(ctx->get_saved_variables(), ctx->saved_data["ignore"].toInt(), 1, {}, grads[0], ready), {}, {}, {}, {}, {}, {}, {}, {}, {}};
   }

@@ -103,3 +103,48 @@ def test_second_derivatives_are_refused_not_lost(losses, name):
     call(h * head).backward()
     assert torch.equal(first, head.grad)
     head.grad = None
+
+
+# ---- the policy loss's gradient between its passes ----------------------------------------------------------------------
+def test_hooks_on_saved_tensors_see_the_waiting_gradient(losses):
+    """The gradient that the policy loss's forward pass leaves is as large as the logits: it can be moved away until it is needed."""
+    x, y, a, b = _data((4, 64, 5003))
+    x.requires_grad_(True)
+    call = _calls(losses, y, a, b)["policy"]
+    size = x.numel() * x.element_size()
+    for factor in (1.0, 3.0):
+        (want,) = torch.autograd.grad(factor * call(x), x)
+        shapes = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: shapes.append(t.shape) or t, lambda t: t):
+            loss = factor * call(x)
+        assert shapes.count(x.shape) == 2              # the logits and their gradient
+        assert torch.equal(torch.autograd.grad(loss, x, retain_graph=True)[0], want)
+        assert torch.equal(torch.autograd.grad(loss, x)[0], want)          # written anew
+        before = torch.cuda.memory_allocated()
+        with torch.autograd.graph.save_on_cpu():
+            loss = factor * call(x)
+        assert torch.cuda.memory_allocated() - before < size // 2
+        assert torch.equal(torch.autograd.grad(loss, x, retain_graph=True)[0], want)
+        assert torch.equal(torch.autograd.grad(loss, x)[0], want)
+    for back in (lambda t: t.half(), lambda t: t.cpu(), lambda t: t[:1], lambda t: t[..., :-1], lambda t: t.cpu() if t.dtype == torch.float32 else t):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: back(t) if t.shape == x.shape and t is not x else t):
+            loss = call(x)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(3 * loss, x)
+    # rows that come back in another order of memory
+    def transposed(t):
+        return t.transpose(1, 2).contiguous().transpose(1, 2) if t.shape == x.shape else t
+    for move in (transposed, lambda t: t.transpose(0, 1).contiguous().transpose(0, 1) if t.shape == x.shape else t):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, move):
+            loss = 3.0 * call(x)
+        assert torch.equal(torch.autograd.grad(loss, x)[0], want)
+
+
+def test_losses_inside_a_checkpoint(losses):
+    from torch.utils.checkpoint import checkpoint
+    x, y, a, b = _data()
+    for name, call in _calls(losses, y, a, b).items():
+        x.requires_grad_(True)
+        (want,) = torch.autograd.grad(call(x * 1.5), x)
+        loss = checkpoint(lambda t: call(t * 1.5), x, use_reentrant=False)
+        assert torch.equal(torch.autograd.grad(loss, x)[0], want), name

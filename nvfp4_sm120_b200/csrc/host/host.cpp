@@ -383,6 +383,7 @@ void check_param(const at::Tensor& p, c10::optional<c10::Device>& dev) {
   dev = p.device();
   if (p.scalar_type() != at::kFloat && p.scalar_type() != at::kBFloat16)
     raise(PyExc_ValueError, std::string("parameters are fp32 or bf16, got ") + c10::toString(p.scalar_type()));
+  if (p.is_neg()) raise(PyExc_ValueError, "a parameter must not be a lazily negated view");
   if (p.layout() != at::kStrided || !p.is_non_overlapping_and_dense())
     raise(PyExc_ValueError, "parameters must fill their memory without gaps or overlaps");
 }
@@ -583,7 +584,7 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
       device_of({&anchor, &*norm_in});
       if (norm_in->scalar_type() != at::kFloat || norm_in->numel() != 1)
         raise(PyExc_ValueError, "grad_norm must be one fp32 element");
-      norm = *norm_in;
+      norm = norm_in->resolve_neg();
       norm_p = float_ptr(norm);
     } else {
       parts = grads.parts(*dev);
@@ -657,7 +658,7 @@ struct Logits {
     dev = device_of({&logits, &labels_in});
     x = logits.resolve_neg();
     if (x.stride(-1) != 1 && x.size(-1) > 1) x = x.contiguous();
-    labels = labels_in.to(at::kLong).contiguous();
+    labels = labels_in.to(at::kLong).resolve_neg().contiguous();
     const bool three = x.dim() == 3;
     rows = nvfp4_logit_rows{x.data_ptr(), x.scalar_type() == at::kFloat, three ? x.size(0) : 1, x.size(-2), x.size(-1),
                             three ? x.stride(0) : 0, x.stride(-2), labels.data_ptr<int64_t>(), ignore};
@@ -668,7 +669,7 @@ struct Logits {
   at::Tensor vec(const at::Tensor& t, int64_t n, const char* name, at::ScalarType type = at::kFloat) const {
     device_of({&x, &t});
     if (t.numel() != n || !t.is_floating_point()) raise(PyExc_ValueError, std::string(name) + " must hold " + std::to_string(n) + " floating-point values");
-    return t.to(type).contiguous();
+    return t.to(type).resolve_neg().contiguous();
   }
 };
 
@@ -724,8 +725,8 @@ at::Tensor dlogits(const torch::autograd::variable_list& saved, int64_t ignore, 
       kept.numel() != 2 * n + (weight.defined() ? 0 : n / per) || reinterpret_cast<uintptr_t>(kept.data_ptr()) % 8 != 0 ||
       (ready.defined() && (ready.sizes() != in.x.sizes() || ready.scalar_type() != in.x.scalar_type() || ready.device() != in.dev)))
     throw std::runtime_error("what a loss saved for its backward pass came back changed");
-  const at::Tensor w = weight.defined() ? weight.to(at::kFloat).contiguous() : kept,
-                   sc = scale.defined() ? scale.to(at::kFloat) : scale;
+  const at::Tensor w = weight.defined() ? weight.to(at::kFloat).resolve_neg().contiguous() : kept,
+                   sc = scale.defined() ? scale.to(at::kFloat).resolve_neg() : scale;
   const float* wp = float_ptr(w) + (weight.defined() ? 0 : 2 * n);
   at::Tensor out = ready.defined() ? ready.resolve_neg() : gradient_like(saved[0], in);
   if (ready.defined() && ((out.size(-1) > 1 && out.stride(-1) != 1) || !rows_apart(in.rows, batch_stride(out), out.stride(-2))))

@@ -206,3 +206,37 @@ def test_reference_sums_keep_their_precision(losses):
     ints = torch.arange(4, device="cuda")
     with pytest.raises(ValueError, match="floating"):
         losses.preference_loss(x, y, ints)
+
+
+# ---- layouts of the other arguments -------------------------------------------------------------------------------------
+def test_lazily_negated_arguments(losses):
+    """Views that torch negates when they are read (the imaginary part of a conjugate, say) count with their sign."""
+    from nvfp4_sm120_b200 import optim
+    x, y = _randn((2, 5, 31), 1).requires_grad_(True), _labels((2, 5), 31, 2, 0.3)
+    w, adv = _randn((2, 5), 3), _randn((2,), 4)
+    lp = losses.token_logprobs(x, y).detach()
+    neg = lambda t: torch._neg_view(-t)
+    assert neg(w).is_neg() and torch.equal(neg(w), w)
+
+    def results(f):
+        a = losses.token_logprobs(x, f(y))
+        b = losses.preference_loss(x, y, f(adv - 20))
+        c = losses.policy_loss(x, y, f(lp - 0.1), f(adv), f(lp + 0.1), kl_coef=0.1)
+        grads = [torch.autograd.grad(o, x, f(g), retain_graph=True)[0] for o, g in ((a, w), (b[0], adv[0]), (c[0], adv[1]))]
+        return [a, *b, c[0], *c[1].values(), *grads]
+
+    assert all(torch.equal(a, b) for a, b in zip(results(neg), results(lambda t: t)))
+    factor = torch.view_as_complex(torch.tensor([1.0, -2.5], device="cuda")).conj().imag
+    assert factor.is_neg() and torch.equal(torch.autograd.grad(losses.preference_loss(x, y, adv)[0], x, factor)[0],
+                                           torch.autograd.grad(losses.preference_loss(x, y, adv)[0], x, factor.clone().resolve_neg())[0])
+    weights = []
+    for norm in (neg(torch.full((), 10.0, device="cuda")), torch.full((), 10.0, device="cuda")):
+        p = torch.nn.Parameter(torch.ones(5, device="cuda"))
+        p.grad = torch.ones_like(p)
+        optim.AdamW([p], max_norm=1e-7, eps=1e-3).step(grad_norm=norm)
+        weights.append(p.detach())
+    assert torch.equal(*weights)
+    p = torch.nn.Parameter(neg(torch.ones(5, device="cuda")))
+    p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="negated"):
+        optim.AdamW([p]).step()

@@ -665,10 +665,23 @@ struct Logits {
   }
   int64_t count() const { return rows.batch * rows.seq; }
   at::Tensor per_row() const { return at::empty(labels.sizes(), on(dev, at::kFloat)); }
-  // a row or sequence vector as the kernels read it
-  at::Tensor vec(const at::Tensor& t, int64_t n, const char* name, at::ScalarType type = at::kFloat) const {
+  // A vector of `shape` as the kernels read it.  Sizes of 1 and a flat vector are let through; the same number of values in another
+  // shape (transposed, say) would be read in the wrong order.
+  at::Tensor vec(const at::Tensor& t, c10::IntArrayRef shape, const char* name, at::ScalarType type = at::kFloat) const {
     device_of({&x, &t});
-    if (t.numel() != n || !t.is_floating_point()) raise(PyExc_ValueError, std::string(name) + " must hold " + std::to_string(n) + " floating-point values");
+    const auto without_ones = [](c10::IntArrayRef s) {
+      std::vector<int64_t> out;
+      for (int64_t n : s)
+        if (n != 1) out.push_back(n);
+      return out;
+    };
+    int64_t n = 1;
+    for (int64_t s : shape) n *= s;
+    if (t.numel() != n || !t.is_floating_point() || (t.dim() != 1 && without_ones(t.sizes()) != without_ones(shape))) {
+      std::string want = "[";
+      for (int64_t s : shape) want += (want.size() > 1 ? ", " : "") + std::to_string(s);
+      raise(PyExc_ValueError, std::string(name) + " must hold " + std::to_string(n) + " floating-point values, " + want + "]");
+    }
     return t.to(type).resolve_neg().contiguous();
   }
 };
@@ -762,7 +775,8 @@ struct Preference : torch::autograd::Function<Preference> {
     const Logits in(logits, labels, ignore);
     if (logits.dim() != 3 || in.rows.batch % 2 != 0)
       raise(PyExc_ValueError, "logits must be [2 pairs, seq, vocab], the chosen sequences first");
-    const at::Tensor r = in.vec(ref, in.rows.batch, "ref_logps", at::kDouble);
+    const bool halves = ref.dim() == 2 && ref.size(0) == 2;                        // [2, pairs]: they lie in the same order
+    const at::Tensor r = in.vec(halves ? ref.reshape({-1}) : ref, {in.rows.batch}, "ref_logps", at::kDouble);
     const c10::cuda::CUDAGuard guard(in.dev);
     const int64_t n = in.count();
     at::Tensor loss = at::empty({}, on(in.dev, at::kFloat)), rewards = at::empty({in.rows.batch}, on(in.dev, at::kFloat)),
@@ -803,10 +817,10 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     const Logits in(logits, labels, ignore);
     const int64_t n = in.count();
     const bool per_sequence = advantages.dim() == 1 && logits.dim() == 3;
-    const at::Tensor old = in.vec(old_logps, n, "old_logps"),
-                     adv = in.vec(advantages, per_sequence ? in.rows.batch : n, "advantages");
+    const at::Tensor old = in.vec(old_logps, labels.sizes(), "old_logps"),
+                     adv = in.vec(advantages, per_sequence ? c10::IntArrayRef(in.rows.batch) : labels.sizes(), "advantages");
     at::Tensor rf, grad;
-    if (ref.has_value()) rf = in.vec(*ref, n, "ref_logps");
+    if (ref.has_value()) rf = in.vec(*ref, labels.sizes(), "ref_logps");
     const c10::cuda::CUDAGuard guard(in.dev);
     at::Tensor logp = in.per_row(), kept = at::empty({3 * n}, on(in.dev, at::kFloat)), loss = at::empty({}, on(in.dev, at::kFloat)),
                stats = at::empty({2}, on(in.dev, at::kFloat));

@@ -240,3 +240,29 @@ def test_lazily_negated_arguments(losses):
     p.grad = torch.ones_like(p)
     with pytest.raises(ValueError, match="negated"):
         optim.AdamW([p]).step()
+
+
+def test_vectors_of_another_shape_are_refused(losses):
+    """As many values as there should be, in another order."""
+    x, y = _randn((6, 4, 31), 1), _labels((6, 4), 31, 2, 0.3)
+    per_label, per_sequence = _randn((6, 4), 3), _randn((6,), 4)
+    want = losses.policy_loss(x, y, per_label, per_sequence, per_label, kl_coef=0.1)[0]
+    token = losses.policy_loss(x, y, per_label, per_label)[0]
+    for bad in (per_label.t(), per_label.view(4, 6), per_label.view(2, 3, 4), per_label.view(3, 8)):
+        for call in (lambda: losses.policy_loss(x, y, bad, per_sequence), lambda: losses.policy_loss(x, y, per_label, bad),
+                     lambda: losses.policy_loss(x, y, per_label, per_sequence, bad, kl_coef=0.1)):
+            with pytest.raises(ValueError, match="must hold 24"):
+                call()
+    for good in (per_label[..., None], per_label[None], per_label.flatten(), per_label.double(), per_label.t().contiguous().t()):
+        assert torch.equal(losses.policy_loss(x, y, good, per_sequence, good, kl_coef=0.1)[0], want)
+    assert torch.equal(losses.policy_loss(x, y, per_label, per_label[..., None])[0], token)
+    assert torch.equal(losses.policy_loss(x.flatten(0, 1), y.flatten(), per_label.flatten(), per_label.flatten())[0], token)
+    loss = losses.preference_loss(x, y, per_sequence)[0]
+    for bad in (per_sequence.view(3, 2), per_sequence.view(2, 3).t()):
+        with pytest.raises(ValueError, match="must hold 6"):
+            losses.preference_loss(x, y, bad)
+    for good in (per_sequence[:, None], per_sequence[None], per_sequence.view(2, 3), per_sequence.bfloat16().double()):
+        assert torch.equal(losses.preference_loss(x, y, good)[0], loss) or good.dtype == torch.float64
+    one, label = _randn((2, 1, 31), 5), _labels((2, 1), 31, 6)
+    assert torch.isfinite(losses.preference_loss(one, label, per_sequence[:2])[0])
+    assert torch.isfinite(losses.policy_loss(one[:1], label[:1], per_label[:1, :1], per_sequence[:1], per_label[:1, 0])[0])

@@ -104,6 +104,23 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """The state of this class (same state_bits), or of a torch.optim.AdamW when state_bits is 32."""
+        pairs = []                                         # (saved state, its parameter) by group
+
+        def take(_, state_dict):                           # behind the other pre-hooks, which may change what is loaded
+            pairs.extend(self._saved_pairs(state_dict))
+            return {**state_dict, "state": {}}             # (torch would cast the moments to the parameters' dtype)
+
+        def place(_):                                      # in front of the other post-hooks, which look at the loaded state
+            self._place(pairs)
+
+        hooks = (self.register_load_state_dict_pre_hook(take), self.register_load_state_dict_post_hook(place, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _saved_pairs(self, state_dict):
         groups = state_dict["param_groups"]
         for g in groups:
             if g.get("amsgrad") or g.get("maximize"):
@@ -125,7 +142,10 @@ class AdamW(torch.optim.Optimizer):
                 fits = p.numel() if self.state_bits == 32 else blocks if n.endswith("_scale") else blocks * BLOCK
                 if st[n].numel() != fits or (self.state_bits == 8 and st[n].dtype != _dtype8(n)):
                     raise ValueError(f"the saved {n} does not fit a parameter of shape {tuple(p.shape)}")
-        super().load_state_dict({"state": {}, "param_groups": groups})
+        return pairs
+
+    def _place(self, pairs):
+        names = _NAMES[self.state_bits]
         self._flat = []
         to, source = [], []
         for group in pairs:

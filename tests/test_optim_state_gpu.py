@@ -1,0 +1,70 @@
+"""State of the multi-tensor AdamW (optim.py): hooks around loading, layouts, what a program may do to it between steps."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BLOCK = 256
+HYPER = dict(lr=3e-3, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1)
+
+
+@pytest.fixture(scope="module")
+def optim():
+    from nvfp4_sm120_b200 import optim as module
+    return module
+
+
+def _params(shapes, dtype=torch.float32, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    out = []
+    for s in shapes:
+        p = torch.nn.Parameter((0.02 * torch.randn(s, device="cuda", generator=gen)).to(dtype))
+        p.grad = (1e-3 * torch.randn(s, device="cuda", generator=gen)).to(dtype)
+        out.append(p)
+    return out
+
+
+def _same(a, b):
+    return a == b if not isinstance(a, torch.Tensor) else torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+# ---- hooks --------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bits", [32, 8])
+def test_hooks_around_loading(optim, bits):
+    """What pre-hooks make of the saved dict is what is loaded, and post-hooks find it in place."""
+    p, q = _params([(33, 7), (300,)]), _params([(33, 7), (300,)])
+    x, y = optim.AdamW(p, **HYPER, state_bits=bits), optim.AdamW(q, **HYPER, state_bits=bits)
+    x.step()
+    x.step()
+    seen = []
+
+    def forget_the_second(opt, saved):
+        seen.append("before")
+        state = {0: {**saved["state"][0], "step": 7}}
+        return {"state": state, "param_groups": [{**g, "lr": 0.5} for g in saved["param_groups"]]}
+
+    def look(opt):
+        assert len(opt.state) == 1 and opt.state[q[0]]["step"] == 7 and opt.param_groups[0]["lr"] == 0.5
+        for name, t in x.state[p[0]].items():
+            assert name == "step" or _same(opt.state[q[0]][name], t)
+        seen.append("after")
+
+    y.register_load_state_dict_pre_hook(forget_the_second)
+    y.register_load_state_dict_post_hook(look)
+    y.load_state_dict(x.state_dict())
+    assert seen == ["before", "after"]
+    y.load_state_dict(x.state_dict())                  # nothing of the first call is left behind
+    assert seen == ["before", "after"] * 2
+    y.step()
+    assert y.state[q[0]]["step"] == 8 and y.state[q[1]]["step"] == 1
+    # a pre-hook that spoils the state is refused before anything changes, and leaves no hook either
+    z = optim.AdamW(q, **HYPER, state_bits=bits)
+    spoil = z.register_load_state_dict_pre_hook(lambda opt, saved: {**saved, "state": {0: {"step": 1}}})
+    with pytest.raises(ValueError, match=f"{bits}-bit"):
+        z.load_state_dict(x.state_dict())
+    assert not z.state
+    spoil.remove()
+    z.load_state_dict(x.state_dict())
+    assert z.state[q[1]]["step"] == 2

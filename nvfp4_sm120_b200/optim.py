@@ -19,6 +19,11 @@ def _dtype8(name):
     return torch.float8_e8m0fnu if name.endswith("_scale") else torch.float8_e4m3fn
 
 
+def _same_order(strides, p):
+    """Are `strides` those of `p`, where they matter?  (Those of sizes of 1 do not.)"""
+    return len(strides) == p.dim() and all(n == 1 or a == b for a, b, n in zip(strides, p.stride(), p.shape))
+
+
 def grad_norm(params):
     """2-norm of the gradients of `params` (an iterable of tensors; those without a gradient are skipped) as an fp32
     0-dim CUDA tensor, summed in 64 bits and in a fixed order.  No host synchronisation."""
@@ -135,7 +140,7 @@ class AdamW(torch.optim.Optimizer):
         pairs = [[(saved[i], p) for i, p in zip(old["params"], new["params"]) if i in saved]
                  for old, new in zip(groups, self.param_groups)]
         for st, p in (pair for group in pairs for pair in group):
-            if "layout" in st and tuple(st["layout"]) != tuple(p.stride()):
+            if "layout" in st and not _same_order(st["layout"], p):
                 raise ValueError(f"the saved moments are in the order of strides {tuple(st['layout'])}, not {p.stride()}")
             blocks = -(-p.numel() // BLOCK)
             for n in names:

@@ -68,3 +68,28 @@ def test_hooks_around_loading(optim, bits):
     spoil.remove()
     z.load_state_dict(x.state_dict())
     assert z.state[q[1]]["step"] == 2
+
+
+# ---- layouts ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bits", [32, 8])
+def test_strides_of_sizes_of_one_do_not_count(optim, bits):
+    """A [1, n] parameter may have any stride along its first dimension: the step takes it, and so does loading."""
+    a = _params([(1, 300), (5, 1, 7)])
+    x = optim.AdamW(a, **HYPER, state_bits=bits)
+    x.step()
+    b = [torch.nn.Parameter(a[0].detach().clone().as_strided((1, 300), (1, 1))),
+         torch.nn.Parameter(a[1].detach().clone().as_strided((5, 1, 7), (7, 1, 1)))]
+    for p, q in zip(a, b):
+        assert p.stride() != q.stride()
+        q.grad = p.grad.clone()
+    y = optim.AdamW(b, **HYPER, state_bits=bits)
+    y.load_state_dict(x.state_dict())
+    for _ in range(2):
+        x.step()
+        y.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    if bits == 8:                                      # an order that matters is refused as ever, whatever its number of sizes
+        t = torch.nn.Parameter(torch.ones(5, 1, 7, device="cuda").permute(2, 1, 0).contiguous().permute(2, 1, 0))
+        for other in (t, torch.nn.Parameter(torch.ones(35, device="cuda"))):
+            with pytest.raises(ValueError, match="order"):
+                optim.AdamW([b[0], other], state_bits=8).load_state_dict(x.state_dict())

@@ -531,8 +531,9 @@ py::object adamw_step(const py::list& groups, const py::dict& state, int bits, c
       check_param(p, dev);
       at::Tensor g = grad_like(p, g0);
       PyObject* st = states.find(ph.ptr());
-      if (st == nullptr) return py::str(captured() ? "capture" : "state");
-      if (!PyDict_Check(st)) raise(PyExc_TypeError, "optimizer state holds dicts");
+      if (st != nullptr && !PyDict_Check(st)) raise(PyExc_TypeError, "optimizer state holds dicts");
+      // (an empty dict is what looking up a parameter in the optimizer's state leaves there)
+      if (st == nullptr || PyDict_GET_SIZE(st) == 0) return py::str(captured() ? "capture" : "state");
       Item it{};
       it.t.param = p.data_ptr();
       it.t.grad = g.data_ptr();

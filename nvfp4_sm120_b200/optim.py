@@ -132,7 +132,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("amsgrad and maximize are not supported")
             if g["weight_decay"] and not g.get("decoupled_weight_decay", True):
                 raise ValueError("the saved state is that of an optimizer whose weight decay is part of the gradient")
-        saved = state_dict["state"]
+        saved = {i: st for i, st in state_dict["state"].items() if st}          # (empty: looked up before its first step)
         names = _NAMES[self.state_bits]
         for i, st in saved.items():
             if any(n not in st for n in ("step", *names)):
@@ -181,7 +181,7 @@ class AdamW(torch.optim.Optimizer):
         if isinstance(done, str) and done == "state":
             for g in self.param_groups:
                 self._make_state([p for p in g["params"]
-                                  if p not in self.state and p.numel() and (p.requires_grad or p.grad is not None)])
+                                  if not self.state.get(p) and p.numel() and (p.requires_grad or p.grad is not None)])
             done = call()
         if isinstance(done, str):
             raise _lib.NVFP4Error("AdamW.step cannot be captured into a CUDA graph: its step count lives on the host")

@@ -93,3 +93,27 @@ def test_strides_of_sizes_of_one_do_not_count(optim, bits):
         for other in (t, torch.nn.Parameter(torch.ones(35, device="cuda"))):
             with pytest.raises(ValueError, match="order"):
                 optim.AdamW([b[0], other], state_bits=8).load_state_dict(x.state_dict())
+
+
+# ---- what a program does between steps ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("bits", [32, 8])
+def test_looking_up_a_parameter_before_its_first_step(optim, bits):
+    """`opt.state[p]` puts an empty dict there, which the first step takes for no state, as torch's optimizers do."""
+    a, b = _params([(33, 7), (300,)]), _params([(33, 7), (300,)])
+    x, y = optim.AdamW(a, **HYPER, state_bits=bits), optim.AdamW(b, **HYPER, state_bits=bits)
+    assert all(len(x.state[p]) == 0 for p in a)
+    late, a[1].grad = a[1].grad, None
+    x.step()
+    saved = x.state_dict()                             # holds the empty dict of the parameter without a gradient
+    assert len(saved["state"]) == 2 and len(saved["state"][1]) == 0
+    x.load_state_dict(saved)
+    assert a[1] not in x.state and x.state[a[0]]["step"] == 1
+    a[1].grad = late
+    for _ in range(2):
+        x.step()
+    b[1].grad = None
+    y.step()
+    b[1].grad = late
+    for _ in range(2):
+        y.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b))

@@ -30,7 +30,7 @@ def grad_norm(params):
     params = [params] if isinstance(params, torch.Tensor) else list(params)
     norm = _lib.host().grad_norm(params)
     if norm is None:
-        return torch.zeros((), device=params[0].device if params else "cuda")
+        return torch.zeros((), dtype=torch.float32, device=params[0].device if params else "cuda")
     return norm
 
 

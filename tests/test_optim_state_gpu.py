@@ -117,3 +117,17 @@ def test_looking_up_a_parameter_before_its_first_step(optim, bits):
     for _ in range(2):
         y.step()
     assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_norm_without_gradients_is_fp32_whatever_the_default(optim):
+    p = torch.nn.Parameter(torch.ones(3, device="cuda"))
+    before = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(torch.float64)
+        got = optim.grad_norm([p])
+    finally:
+        torch.set_default_dtype(before)
+    assert got.dtype == torch.float32 and got.device == p.device and float(got) == 0.0
+    opt = optim.AdamW([p], max_norm=1.0)
+    p.grad = torch.ones_like(p)
+    opt.step(grad_norm=got)                            # and so it can be handed on

@@ -162,7 +162,8 @@ class GPT(nn.Module):
     def token_logprobs(self, idx, targets, ignore_index=losses.IGNORE_INDEX):
         """Log-probabilities of `targets` [batch, seq] after each prefix of `idx`, fp32, 0 where a target is ignored
         (losses.token_logprobs; CUDA only)."""
-        return losses.token_logprobs(GPT.forward(self, idx)[0], targets, ignore_index)
+        out = self(idx)                            # through __call__: hooks on the model run, and a subclass has its own forward
+        return losses.token_logprobs(out[0] if isinstance(out, tuple) else out, targets, ignore_index)
 
     def num_params(self):
         """Non-embedding parameter count (the tied head counts once, as the embedding)."""

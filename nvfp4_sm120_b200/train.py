@@ -12,7 +12,7 @@ the same vocabulary and sequence format; the loss floor is the entropy of that d
 
 --optimizer: torch (torch.optim.AdamW after clip_grad_norm_, the default), adamw or adamw8 (optim.AdamW with 32- or 8-bit
 moments, clipping inside its step).  --objective: lm (cross-entropy, the default); preference (losses.preference_loss on pairs
-of sequences that share their first half) or policy (losses.policy_loss on sequences scored by a fixed reward, advantages
+of sequences that share their first half; the batch sizes count pairs) or policy (losses.policy_loss on sequences scored by a fixed reward, advantages
 normalized over the microbatch), both against a frozen copy of the initial model.
 Every rank prints nothing; rank 0 prints one JSON line per logged step and a final summary."""
 from __future__ import annotations
@@ -97,6 +97,8 @@ class Trainer:
         self.micro_batch, self.accum = micro_batch, per_rank // micro_batch
         self.reducer = parallel.GradientReducer(self.params, group) if (world > 1 and overlap) else None
         self.group = group
+        # of all ranks; a preference step takes two sequences for each one that the batch sizes count
+        self.tokens_per_step = global_batch * seq * (2 if objective == "preference" else 1)
 
     def step(self, step):
         """Optimizer step number `step` (1-based); returns this rank's mean microbatch loss (a tensor)."""
@@ -165,8 +167,8 @@ def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--backend", default="fp4", choices=["fp4", "bf16"])
     ap.add_argument("--steps", type=int, default=300)
-    ap.add_argument("--global-batch", type=int, default=256, help="sequences per optimizer step, all ranks")
-    ap.add_argument("--micro-batch", type=int, default=16, help="sequences per forward/backward")
+    ap.add_argument("--global-batch", type=int, default=256, help="sequences (pairs with --objective preference) per optimizer step, all ranks")
+    ap.add_argument("--micro-batch", type=int, default=16, help="sequences (or pairs) per forward/backward")
     ap.add_argument("--seq", type=int, default=1024)
     ap.add_argument("--dim", type=int, default=768)
     ap.add_argument("--layers", type=int, default=12)
@@ -203,7 +205,7 @@ def main():
 
     emit({"event": "start", "backend": a.backend, "optimizer": a.optimizer, "objective": a.objective,
           "params_non_embedding": tr.model.num_params(), "world": world,
-          "tokens_per_step": a.global_batch * a.seq, "fp4_linears": len(tr.model.fp4_linears()),
+          "tokens_per_step": tr.tokens_per_step, "fp4_linears": len(tr.model.fp4_linears()),
           "zipf_entropy_nats": tr.entropy})
     t_start = None
     loss_sum = torch.zeros((), device=dev)
@@ -221,7 +223,7 @@ def main():
     dt = time.perf_counter() - t_start if t_start else float("nan")
     steps_timed = max(1, a.steps - 2)
     emit({"event": "done", "backend": a.backend, "world": world, "steps": a.steps,
-          "ms_per_step": dt / steps_timed * 1e3, "tokens_per_s": a.global_batch * a.seq * steps_timed / dt,
+          "ms_per_step": dt / steps_timed * 1e3, "tokens_per_s": tr.tokens_per_step * steps_timed / dt,
           "final_loss": round(float(loss_sum), 4)})
     if world > 1:
         dist.destroy_process_group()

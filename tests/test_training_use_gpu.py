@@ -46,3 +46,26 @@ def test_scores_go_through_the_models_call():
     torch.manual_seed(0)
     lm = LM(61, 64, 2, 4, 4, 16, 128, False)
     assert torch.equal(lm.token_logprobs(x, y), losses.token_logprobs(lm(x), y))
+
+
+@pytest.mark.parametrize("objective,per_count", [("lm", 1), ("preference", 2), ("policy", 1)])
+def test_reported_tokens_are_those_trained_on(objective, per_count, monkeypatch, tmp_path):
+    from nvfp4_sm120_b200 import train
+    trained = []
+    step = train.Trainer.step
+
+    def counted(self, n):
+        hook = self.model.register_forward_pre_hook(lambda m, args: trained.append(args[0].numel()) if torch.is_grad_enabled() else None)
+        loss = step(self, n)
+        hook.remove()
+        return loss
+
+    monkeypatch.setattr(train.Trainer, "step", counted)
+    out = tmp_path / "log.jsonl"
+    monkeypatch.setattr(sys, "argv", ["train", "--steps", "4", "--backend", "bf16", "--vocab", "199", "--dim", "64", "--layers", "2", "--heads", "4",
+                                      "--seq", "32", "--global-batch", "8", "--micro-batch", "4", "--objective", objective, "--out", str(out)])
+    train.main()
+    log = [json.loads(line) for line in open(out)]
+    start, done = log[0], log[-1]
+    assert start["tokens_per_step"] * 4 == sum(trained) == 4 * 8 * 32 * per_count
+    assert abs(done["tokens_per_s"] * done["ms_per_step"] * 1e-3 - start["tokens_per_step"]) <= 1e-6 * start["tokens_per_step"]

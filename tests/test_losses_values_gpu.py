@@ -266,3 +266,68 @@ def test_vectors_of_another_shape_are_refused(losses):
     one, label = _randn((2, 1, 31), 5), _labels((2, 1), 31, 6)
     assert torch.isfinite(losses.preference_loss(one, label, per_sequence[:2])[0])
     assert torch.isfinite(losses.policy_loss(one[:1], label[:1], per_label[:1, :1], per_sequence[:1], per_label[:1, 0])[0])
+
+
+# ---- sizes --------------------------------------------------------------------------------------------------------------
+def _softmax_gradient(x, y, w, rows=64):
+    """w (onehot - softmax) of [rows, vocab] logits in 64 bits, in pieces: (index of the first row, gradient, softmax)."""
+    for i in range(0, x.shape[0], rows):
+        p = torch.softmax(x[i:i + rows].double(), 1)
+        d = torch.where(y[i:i + rows] == IGNORE, 0.0, w[i:i + rows].double())[:, None]
+        yield i, (-d * p).scatter_add(1, y[i:i + rows].clamp(min=0)[:, None], d), d.abs() * p
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(600, 131073, torch.float32), (400, 250007, torch.bfloat16)])
+def test_policy_with_rows_that_the_cache_cannot_hold(losses, rows, vocab, dtype):
+    """All rows in flight are more than the L2 holds: the second read of a row comes from memory."""
+    x, y = (2 * _randn((rows, vocab), 1)).to(dtype), _labels((rows,), vocab, 2, 0.3)
+    lp = torch.cat([torch.log_softmax(x[i:i + 64].double(), 1).gather(1, y[i:i + 64].clamp(min=0)[:, None]) for i in range(0, rows, 64)])[:, 0]
+    adv = _randn((rows,), 3)
+    x.requires_grad_(True)
+    loss, stats = losses.policy_loss(x, y, (lp - math.log(1.1)).float(), adv)
+    n = int((y != IGNORE).sum())
+    live = y != IGNORE
+    # logp: sums of 64 terms a thread, joined 13 times, 2^-22 of ex2.approx; its rounding of some 20.  Ratio 1.1 within the clamp.
+    err = (64 + 13 + 4 + 8) * U + 2.0 ** -22 + 20 * U
+    assert ((stats["logps"] - lp).abs()[live] <= err).all() and (stats["logps"][~live] == 0).all()
+    assert abs(loss.item() + 1.1 * (adv.double() * live).sum().item() / n) <= 2 * 1.1 * float(adv.abs().max()) * (err + 20 * U)
+    (g,) = torch.autograd.grad(loss, x)
+    w = -1.1 * adv / n
+    rel = err + 2.0 ** -22 + 40 * U + err + 20 * U        # of p: the sum's, ex2's, the exponents'; of w: the ratio's
+    for i, want, size in _softmax_gradient(x.detach(), y, w):
+        got = g[i:i + 64].double()
+        off = size * rel + torch.finfo(dtype).eps / 2 * 1.001 * want.abs() + (err + 20 * U) * want.abs() + 2.0 ** -126
+        assert ((got - want).abs() <= off).all()
+
+
+@pytest.mark.parametrize("name", ["preference", "policy"])
+def test_more_logits_than_32_bits_count_in_a_loss(losses, name):
+    seq, vocab = 21400, 50257
+    assert 2 * seq * vocab > 2 ** 31
+    x = torch.zeros(2, seq, vocab, dtype=torch.bfloat16, device="cuda")
+    some = torch.tensor([0, 17, seq // 2, seq - 2, seq - 1], device="cuda")
+    x[1, some] = (3 * _randn((5, vocab), 7)).bfloat16()
+    x.requires_grad_(True)
+    y = torch.full((2, seq), IGNORE, device="cuda")
+    y[1, some] = torch.tensor([0, 5, vocab - 1, 9, vocab - 1], device="cuda")
+    part = x.detach()[1, some]
+    lp = torch.log_softmax(part.double(), 1).gather(1, y[1, some][:, None])[:, 0]
+    if name == "preference":
+        # L_0 = 0, h = beta (0 - (L_1 - ref)); dloss / dL_1 = beta sigmoid(-h)
+        ref = torch.stack((torch.zeros_like(lp[0]), lp.sum() - 0.3))
+        loss, chosen, rejected = losses.preference_loss(x, y, ref, beta=1.0)
+        assert abs(float(rejected) - 0.3) <= 2.0 ** -18 and float(chosen) == 0.0
+        w = torch.full((5,), 1 / (1 + math.exp(-0.3)), device="cuda")
+    else:
+        old, adv = torch.zeros(2, seq, device="cuda"), torch.tensor([0.0, 1.5], device="cuda")
+        old[1, some] = (lp + 0.1).float()
+        loss, stats = losses.policy_loss(x, y, old, adv)
+        w = torch.full((5,), -1.5 * math.exp(-0.1) / 5, device="cuda")
+    (g,) = torch.autograd.grad(loss, x)
+    ((_, want, size),) = _softmax_gradient(part, y[1, some], w)
+    # bf16's rounding, and 2^-18 for sums, exponents and w together
+    assert ((g[1, some].double() - want).abs() <= 2.0 ** -18 * (size + want.abs()) + 2.0 ** -9 * 1.001 * 2 * want.abs() + 2.0 ** -126).all()
+    assert torch.count_nonzero(g[0]) == 0 and torch.count_nonzero(g[1, 18:seq // 2]) == 0 and torch.count_nonzero(g[1, 1:17]) == 0
+    assert torch.count_nonzero(g[1, seq // 2 + 1:seq - 2]) == 0
+    del x, g
+    torch.cuda.empty_cache()

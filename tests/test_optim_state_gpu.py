@@ -132,3 +132,69 @@ def test_norm_without_gradients_is_fp32_whatever_the_default(optim):
     opt = optim.AdamW([p], max_norm=1.0)
     p.grad = torch.ones_like(p)
     opt.step(grad_norm=got)                            # and so it can be handed on
+
+
+# ---- layouts and sizes of the 32-bit step -------------------------------------------------------------------------------
+def _operations(p, g, m, v, t, lr, b1, b2, eps, wd):
+    """One step in fp32, one torch operation for each."""
+    g, pf = g.float(), p.float()
+    m = m * b1 + g * (1 - b1)
+    v = v * b2 + (g * (1 - b2)) * g
+    ratio = m / (v.sqrt() * (1 / math.sqrt(1 - b2 ** t)) + eps)
+    return (pf * (1 - lr * wd) - ratio * (lr / (1 - b1 ** t))).to(p.dtype), m, v
+
+
+def test_both_moments_in_every_layout_and_what_lies_around(optim):
+    """Another memory order, no vector alignment, channels last, missing gradients: weights and both moments have the bits of the torch
+    operations, and nothing around a parameter that is a part of a buffer is written."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=gen)
+    buf = rand(5001)
+    around = buf.clone()
+    params = [torch.nn.Parameter(rand(40, 70).t()), torch.nn.Parameter(buf[1:4097]), torch.nn.Parameter(rand(300)),
+              torch.nn.Parameter(rand(6, 5, 4, 3).to(memory_format=torch.channels_last))]
+    opt = optim.AdamW(params, **HYPER)
+    model = [[p.detach().clone(), torch.zeros_like(p), torch.zeros_like(p), 0] for p in params]
+    for k in range(4):
+        for i, p in enumerate(params):
+            p.grad = None
+            if (k + i) % 3 != 0:
+                g = rand(*p.shape)
+                p.grad = g.contiguous()
+                w, m, v, t = model[i]
+                model[i] = [*_operations(w, g, m, v, t + 1, 3e-3, 0.9, 0.95, 1e-8, 0.1), t + 1]
+        opt.step()
+    for p, (w, m, v, t) in zip(params, model):
+        st = opt.state[p]
+        assert torch.equal(p.detach(), w) and torch.equal(st["exp_avg"], m) and torch.equal(st["exp_avg_sq"], v) and st["step"] == t
+    assert torch.equal(buf[:1], around[:1]) and torch.equal(buf[4097:], around[4097:]) and not torch.equal(buf[1:4097], around[1:4097])
+
+
+def test_more_elements_than_32_bits_count_with_32_bit_moments(optim):
+    n = 2 ** 31 + 300
+    p = torch.nn.Parameter(torch.ones(n, dtype=torch.bfloat16, device="cuda"))
+    p.grad = torch.zeros_like(p)
+    ends = torch.tensor([0, 255, 256, n // 2, n - 301, n - 45, n - 1], device="cuda")
+    p.grad[ends] = 2.0
+    opt = optim.AdamW([p], lr=0.5, weight_decay=0.0, max_norm=1e9)
+    opt.step()
+    # the gradient's sign at the first step, within the roundings of the update and of bf16 (0.5 is a bf16 number)
+    assert ((p.detach()[ends].float() - 0.5).abs() <= 2.0 ** -8).all() and int((p.detach() != 1).sum()) == len(ends)
+    st = opt.state[p]
+    for name, want in (("exp_avg", 0.1 * 2), ("exp_avg_sq", 0.001 * 4)):
+        assert (st[name][ends] - want).abs().max() <= 4 * 2.0 ** -24 * want and int(torch.count_nonzero(st[name])) == len(ends)
+    del p, opt, st
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_saved_state_loads_with_torch_loads_defaults(optim, bits, tmp_path):
+    """Tensors, numbers and tuples alone: no pickled code."""
+    a = _params([(33, 77), (1, 5)])
+    x = optim.AdamW(a, **HYPER, state_bits=bits, max_norm=1.0)
+    x.step()
+    torch.save(x.state_dict(), tmp_path / "state.pt")
+    y = optim.AdamW(a, **HYPER, state_bits=bits, max_norm=1.0)
+    y.load_state_dict(torch.load(tmp_path / "state.pt"))
+    for p in a:
+        assert all(_same(t, y.state[p][name]) for name, t in x.state[p].items())

@@ -384,6 +384,8 @@ void check_param(const at::Tensor& p, c10::optional<c10::Device>& dev) {
   if (p.scalar_type() != at::kFloat && p.scalar_type() != at::kBFloat16)
     raise(PyExc_ValueError, std::string("parameters are fp32 or bf16, got ") + c10::toString(p.scalar_type()));
   if (p.is_neg()) raise(PyExc_ValueError, "a parameter must not be a lazily negated view");
+  if (p.is_inference() && !c10::InferenceMode::is_enabled())
+    raise(PyExc_ValueError, "a parameter made in inference mode cannot be changed outside it");
   if (p.layout() != at::kStrided || !p.is_non_overlapping_and_dense())
     raise(PyExc_ValueError, "parameters must fill their memory without gaps or overlaps");
 }
@@ -678,7 +680,7 @@ struct Logits {
     };
     int64_t n = 1;
     for (int64_t s : shape) n *= s;
-    if (t.numel() != n || !t.is_floating_point() || (t.dim() != 1 && without_ones(t.sizes()) != without_ones(shape))) {
+    if (t.numel() != n || !t.is_floating_point() || (t.dim() != 1 && t.sizes() != shape && without_ones(t.sizes()) != without_ones(shape))) {
       std::string want = "[";
       for (int64_t s : shape) want += (want.size() > 1 ? ", " : "") + std::to_string(s);
       raise(PyExc_ValueError, std::string(name) + " must hold " + std::to_string(n) + " floating-point values, " + want + "]");

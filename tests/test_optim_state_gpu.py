@@ -198,3 +198,34 @@ def test_saved_state_loads_with_torch_loads_defaults(optim, bits, tmp_path):
     y.load_state_dict(torch.load(tmp_path / "state.pt"))
     for p in a:
         assert all(_same(t, y.state[p][name]) for name, t in x.state[p].items())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_made_in_inference_mode(optim, bits):
+    """Refused outside that mode before anything changes, as torch's optimizers refuse them; stepped inside it."""
+    with torch.inference_mode():
+        p = torch.ones(300, device="cuda")
+        p.grad = torch.ones_like(p)
+    (q,) = _params([(300,)])
+    w = q.detach().clone()
+    opt = optim.AdamW([q, p], **HYPER, state_bits=bits)
+    with pytest.raises(ValueError, match="inference"):
+        opt.step()
+    assert torch.equal(q.detach(), w) and torch.equal(p, torch.ones_like(p))
+    assert all(st["step"] == 0 for st in opt.state.values())
+    with torch.inference_mode():
+        opt.step()
+    assert opt.state[p]["step"] == 1 and (p != 1).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_copied_optimizer_loads_state(optim, bits):
+    import copy
+    a = _params([(33, 7), (300,)])
+    x = optim.AdamW(a, **HYPER, state_bits=bits)
+    x.step()
+    b, y = copy.deepcopy((a, x))
+    x.step()
+    y.load_state_dict(x.state_dict())
+    for p, q in zip(a, b):
+        assert y.state[q]["step"] == 2 and all(_same(t, y.state[q][name]) for name, t in x.state[p].items())

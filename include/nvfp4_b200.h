@@ -461,14 +461,17 @@ int nvfp4_logprob_bwd(const nvfp4_logit_rows* rows, const nvfp4_row_stat* stat, 
 
 /*
  * Preference loss of batch / 2 pairs, sequence i chosen over sequence batch / 2 + i: with L_i the sum of the sequence's
- * logp (fp64 here, [batch * seq], as ref [batch] is: a reward is a small difference of long sums),
+ * logp (fp64 here, [batch * seq]: a reward is a small difference of long sums; _ref64 takes ref [batch] in fp64 too),
  * rewards[i] = beta (L_i - ref[i]), h = rewards[chosen] - rewards[rejected],
  * loss = mean(-(1 - label_smoothing) logsigmoid(h) - label_smoothing logsigmoid(-h)).
  * weight[i] = dloss / dL_i, for nvfp4_logprob_bwd with rows_per_weight = seq.  No counterpart in the reference.
  */
-int nvfp4_preference_fwd(const nvfp4_logit_rows* rows, const double* ref, double beta, double label_smoothing, double* logp,
+int nvfp4_preference_fwd(const nvfp4_logit_rows* rows, const float* ref, double beta, double label_smoothing, double* logp,
                          nvfp4_row_stat* stat, float* loss, float* rewards, float* weight, void* workspace, size_t workspace_bytes,
                          void* stream);
+int nvfp4_preference_fwd_ref64(const nvfp4_logit_rows* rows, const double* ref, double beta, double label_smoothing, double* logp,
+                               nvfp4_row_stat* stat, float* loss, float* rewards, float* weight, void* workspace,
+                               size_t workspace_bytes, void* stream);
 
 /*
  * Clipped policy loss with a KL term: rho = exp(logp - old_logp), A = advantage[row / rows_per_advantage], d = ref_logp - logp,

@@ -81,6 +81,8 @@ _SIGS = {
                                      _c.c_int64, _c.c_int64, _c.c_void_p]),
     "nvfp4_preference_fwd": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_double, _c.c_double, _c.c_void_p, _c.c_void_p,
                                         _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "nvfp4_preference_fwd_ref64": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_double, _c.c_double, _c.c_void_p, _c.c_void_p,
+                                              _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
     "nvfp4_policy_fwd": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_double, _c.c_double,
                                     _c.c_double, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
                                     _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_size_t, _c.c_void_p]),

@@ -30,8 +30,8 @@ namespace {
   F(nvfp4_amax_bf16) F(nvfp4_amax_both_bf16) F(nvfp4_quantize_fused_bf16) F(nvfp4_quantize_shard_bf16)                 \
   F(nvfp4_quantize_weight_bf16) F(nvfp4_quantize_dual_bf16) F(nvfp4_round_amax_f32) F(nvfp4_gemm) F(nvfp4_gemm_amax) \
   F(nvfp4_gemm_bf16_as_f32) F(nvfp4_adamw) F(nvfp4_sumsq) F(nvfp4_sumsq_parts) F(nvfp4_norm_of_sumsq)       \
-  F(nvfp4_logprob_fwd) F(nvfp4_logprob_bwd) F(nvfp4_preference_fwd) F(nvfp4_policy_fwd)                         \
-  F(nvfp4_status_string)
+  F(nvfp4_logprob_fwd) F(nvfp4_logprob_bwd) F(nvfp4_preference_fwd) F(nvfp4_preference_fwd_ref64)               \
+  F(nvfp4_policy_fwd) F(nvfp4_status_string)
 
 struct Library {
 #define F(name) decltype(&::name) name = nullptr;
@@ -779,17 +779,22 @@ struct Preference : torch::autograd::Function<Preference> {
     if (logits.dim() != 3 || in.rows.batch % 2 != 0)
       raise(PyExc_ValueError, "logits must be [2 pairs, seq, vocab], the chosen sequences first");
     const bool halves = ref.dim() == 2 && ref.size(0) == 2;                        // [2, pairs]: they lie in the same order
-    const at::Tensor r = in.vec(halves ? ref.reshape({-1}) : ref, {in.rows.batch}, "ref_logps", at::kDouble);
+    const at::Tensor r = in.vec(halves ? ref.reshape({-1}) : ref, {in.rows.batch}, "ref_logps",
+                                    ref.scalar_type() == at::kDouble ? at::kDouble : at::kFloat);
     const c10::cuda::CUDAGuard guard(in.dev);
     const int64_t n = in.count();
     at::Tensor loss = at::empty({}, on(in.dev, at::kFloat)), rewards = at::empty({in.rows.batch}, on(in.dev, at::kFloat)),
                kept = at::empty({2 * n + in.rows.batch}, on(in.dev, at::kFloat));
     const at::Tensor scratch = loss_scratch(in.dev, 8 * n);
     uint8_t* ws = scratch.data_ptr<uint8_t>();
-    check(lib.nvfp4_preference_fwd(&in.rows, r.data_ptr<double>(), beta, smoothing, reinterpret_cast<double*>(ws + NVFP4_LOSS_WORKSPACE),
-                                   stat_ptr(kept), float_ptr(loss), float_ptr(rewards), float_ptr(kept) + 2 * n, ws, NVFP4_LOSS_WORKSPACE,
-                                   stream_of(in.dev)),
-          "nvfp4_preference_fwd");
+    double* logp = reinterpret_cast<double*>(ws + NVFP4_LOSS_WORKSPACE);
+    const auto call = [&](auto entry, const auto* reference) {
+      check(entry(&in.rows, reference, beta, smoothing, logp, stat_ptr(kept), float_ptr(loss), float_ptr(rewards), float_ptr(kept) + 2 * n, ws,
+                  NVFP4_LOSS_WORKSPACE, stream_of(in.dev)),
+            "nvfp4_preference_fwd");
+    };
+    if (r.scalar_type() == at::kDouble) call(lib.nvfp4_preference_fwd_ref64, r.const_data_ptr<double>());
+    else call(lib.nvfp4_preference_fwd, r.const_data_ptr<float>());
     ctx->save_for_backward({logits, labels, kept});
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["seq"] = in.rows.seq;

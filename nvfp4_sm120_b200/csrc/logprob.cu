@@ -396,8 +396,10 @@ template <int N> __device__ __forceinline__ bool grid_sum(double (&v)[N], double
 }
 
 // ---- preference loss ----------------------------------------------------------------------------------------------------
-// One CTA per pair in turn: sums of both sequences in 64 bits (they differ little and are long), rewards, loss, weights.
-__global__ void __launch_bounds__(kThreads) preference_kernel(const double* __restrict__ logp, const double* __restrict__ ref, int64_t pairs,
+// One CTA per pair in turn: sums of both sequences in 64 bits (they differ little and are long), rewards, loss, weights.  The reference
+// comes as it was given, fp32 or fp64: a cast in front would be a launch of its own (78 us instead of 72 for pairs of 12 rows of 13).
+template <class Ref>
+__global__ void __launch_bounds__(kThreads) preference_kernel(const double* __restrict__ logp, const Ref* __restrict__ ref, int64_t pairs,
                                                               uint32_t seq, double beta, double smooth, double* __restrict__ parts,
                                                               unsigned int* __restrict__ ticket, float* __restrict__ loss,
                                                               float* __restrict__ rewards, float* __restrict__ weight) {
@@ -658,15 +660,15 @@ extern "C" int nvfp4_logprob_bwd(const nvfp4_logit_rows* in, const nvfp4_row_sta
   return launched();
 }
 
-extern "C" int nvfp4_preference_fwd(const nvfp4_logit_rows* in, const double* ref, double beta, double label_smoothing, double* logp,
-                                    nvfp4_row_stat* stat, float* loss, float* rewards, float* weight, void* workspace,
-                                    size_t workspace_bytes, void* stream_) {
+template <class Ref>
+static int preference_fwd(const nvfp4_logit_rows* in, const Ref* ref, double beta, double label_smoothing, double* logp, nvfp4_row_stat* stat,
+                          float* loss, float* rewards, float* weight, void* workspace, size_t workspace_bytes, void* stream_) {
   Rows r;
   if (const int code = check_rows(in, r); code != NVFP4_OK) return code;
   if (in->batch % 2 != 0) return NVFP4_E_SHAPE;
   if (!ref || !logp || !stat || !loss || !rewards || !weight || !workspace) return NVFP4_E_NULL;
   if (workspace_bytes < NVFP4_LOSS_WORKSPACE) return NVFP4_E_WORKSPACE;
-  if (!aligned(ref, 8) || !aligned(logp, 8) || !aligned(stat, 8) || !aligned(loss, 4) || !aligned(rewards, 4) || !aligned(weight, 4) ||
+  if (!aligned(ref, sizeof(Ref)) || !aligned(logp, 8) || !aligned(stat, 8) || !aligned(loss, 4) || !aligned(rewards, 4) || !aligned(weight, 4) ||
       !aligned(workspace, 16))
     return NVFP4_E_ALIGN;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
@@ -675,9 +677,20 @@ extern "C" int nvfp4_preference_fwd(const nvfp4_logit_rows* in, const double* re
   forward(r, in->is_f32 != 0, logp, stat, ticket, stream);
   if (const int code = launched(); code != NVFP4_OK) return code;
   const int64_t pairs = in->batch / 2;
-  preference_kernel<<<(unsigned)(pairs < NVFP4_LOSS_PARTS ? pairs : NVFP4_LOSS_PARTS), kThreads, 0, stream>>>(
+  preference_kernel<Ref><<<(unsigned)(pairs < NVFP4_LOSS_PARTS ? pairs : NVFP4_LOSS_PARTS), kThreads, 0, stream>>>(
       logp, ref, pairs, r.seq, beta, label_smoothing, parts, ticket, loss, rewards, weight);
   return launched();
+}
+
+extern "C" int nvfp4_preference_fwd(const nvfp4_logit_rows* in, const float* ref, double beta, double label_smoothing, double* logp,
+                                    nvfp4_row_stat* stat, float* loss, float* rewards, float* weight, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  return preference_fwd(in, ref, beta, label_smoothing, logp, stat, loss, rewards, weight, workspace, workspace_bytes, stream);
+}
+extern "C" int nvfp4_preference_fwd_ref64(const nvfp4_logit_rows* in, const double* ref, double beta, double label_smoothing, double* logp,
+                                          nvfp4_row_stat* stat, float* loss, float* rewards, float* weight, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
+  return preference_fwd(in, ref, beta, label_smoothing, logp, stat, loss, rewards, weight, workspace, workspace_bytes, stream);
 }
 
 extern "C" int nvfp4_policy_fwd(const nvfp4_logit_rows* in, const float* old_logp, const float* advantage,

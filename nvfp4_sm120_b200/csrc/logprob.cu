@@ -16,7 +16,7 @@
 // one mask value) and off by 5e-4 beside one of 1e4, and with it all of the row's gradient.
 // A row belongs to a warp or to a CTA of 128 to 512 threads, by its length and the number of rows (group_of).
 // The policy loss's w depends on its own row alone, so its kernel writes the row's gradient right behind the sum, while
-// the row is in L2: HBM sees each row once.  The preference loss has to see both sequences first; its backward takes the
+// the row is in L2: HBM sees each row once, up to the length that policy_rows tells.  The preference loss has to see both sequences first; its backward takes the
 // rows in the opposite order, so that the last ones read are still in L2.
 #include <cfloat>
 #include <type_traits>
@@ -514,7 +514,7 @@ __device__ __forceinline__ void no_row(const PolicyOut& o, int64_t rows, int64_t
   o.norm[row] = Norm{0.0f, 0.0f};
 }
 
-// One group for each row, which it reads twice when it writes the gradient: the second time from L2.
+// One group for each row, which it reads twice when it writes the gradient: the second time from L2 unless the rows are very long.
 template <class T, int GROUP>
 __global__ void __launch_bounds__(Group<GROUP>::threads) policy_kernel(const Rows r, const Policy p, const Words* __restrict__ words, int parts,
                                                                        const PolicyOut o, const Out<T> grad) {
@@ -616,7 +616,9 @@ static_assert(sizeof(Words) <= kWordsBytes && kWordsBytes + 4 * 8 * NVFP4_LOSS_P
 
 // The row is read again right behind its sum, from L2, with eight vectors of a thread in flight to hide its latency (8192 rows of
 // 50257 bf16, a quarter masked: 276 us, 5.1 TB/s; 317 with two vectors, 285 with four; 309 with the row kept in shared memory and
-// the next one copied in behind it).  The same kernel with and without a gradient: the loss has the same bits.
+// the next one copied in behind it).  The rows in flight, two an SM for long ones, and their gradients have to fit in L2: of 1.6 GB of logits
+// 1.6 GB are read from HBM in rows of up to 131 KB, 2.0 to 2.3 in rows of 200 KB, 2.9 to 3.0 in rows of 262 KB (65536 fp32 logits,
+// 131072 of bf16) and 3.2 beyond: 541, 599, 693 and 725 to 763 us in fp32.  The same kernel with and without a gradient: the loss has the same bits.
 void policy_rows(const Rows& r, bool f32, const Policy& p, Words* words, int counts, const PolicyOut& o, void* dlogits, int64_t dstride_b,
                  int64_t dstride_t, cudaStream_t stream) {
   by_rows(f32, r, true, [&](auto t, auto g, unsigned grid) {

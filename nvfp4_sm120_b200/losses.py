@@ -5,8 +5,12 @@ All take logits [batch, seq, vocab] (or [rows, vocab]; fp32 or bf16, any strides
 the leading shape, already shifted: labels[b, t] is the token that logits[b, t] predict, as in models.GPT.forward(idx,
 targets).  A position whose label is `ignore_index` (prompt, padding) has no part in the result and is not read; any other
 label outside the vocabulary gives NaN.  Empty logits are refused.  Arithmetic is fp32, sums over tokens are 64 bits, the
-gradient is rounded once to the logits' dtype.  Gradients are those of the logits: every other argument is a constant.
-Differentiable once.
+gradient is rounded once to the logits' dtype.  Logits may lie anywhere: a common offset changes nothing, and a row of one finite
+value, whatever it is, has the uniform distribution.  Gradients are those of the logits: every other argument is a constant.
+Differentiable once: a second derivative raises.
+
+All can be captured into a CUDA graph, backward pass included, while no eager graph of the same leaves lives: torch adds up a leaf's
+gradient on the stream that its first living graph was made on.
 
 The reference trains with cross-entropy alone (nvfp4_train.py:159-185)."""
 from __future__ import annotations

@@ -14,7 +14,7 @@ def pytest_configure(config):
 
 # Tests that pin a value which is not the operator's, each with the test that holds the right one.
 _PINS_A_WRONG_VALUE = {
-    "tests/test_losses_gpu.py::test_masked_logits":
+    "test_losses_gpu.py::test_masked_logits":
         "expects log-probability 0 of a label in a row whose logits are all alike (the type's lowest or highest value); log softmax "
         "is -log(vocab) there: tests/test_losses_values_gpu.py::test_masked_rows, test_rows_of_one_value",
 }
@@ -22,7 +22,7 @@ _PINS_A_WRONG_VALUE = {
 
 def pytest_collection_modifyitems(items):
     for item in items:
-        reason = _PINS_A_WRONG_VALUE.get(item.nodeid.split("[")[0])
+        reason = _PINS_A_WRONG_VALUE.get(item.nodeid.split("/")[-1].split("[")[0])
         if reason:
             item.add_marker(pytest.mark.xfail(reason=reason, raises=AssertionError, strict=True))
 

@@ -139,6 +139,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"the saved state of parameter {i} is not that of {self.state_bits}-bit moments")
         pairs = [[(saved[i], p) for i, p in zip(old["params"], new["params"]) if i in saved]
                  for old, new in zip(groups, self.param_groups)]
+        if any(pairs):
+            _lib.cuda_device_of(*(p for group in pairs for _, p in group))
         for st, p in (pair for group in pairs for pair in group):
             if "layout" in st and not _same_order(st["layout"], p):
                 raise ValueError(f"the saved moments are in the order of strides {tuple(st['layout'])}, not {p.stride()}")
